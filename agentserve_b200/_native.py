@@ -67,6 +67,8 @@ SIGNATURES = {
                                                 _P]),
     "as_greedy_workspace_size": (_SZ, [_I32]),
     "as_greedy_argmax": (ctypes.c_int, [_P, _P, _I64, _I32, _I32, _I32, _P, _SZ, _P]),
+    "as_sample_tokens": (ctypes.c_int, [_P, _P, _P, _I64, _P, _P, _P, _P, _P, _I32, _I32, _I32,
+                                        _P]),
     "as_rmsnorm": (ctypes.c_int, [_P, _P, _P, _I64, _I32, _F32, _I32, _P]),
     "as_add_rmsnorm": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I32, _F32, _I32, _P]),
     "as_silu_mul": (ctypes.c_int, [_P, _P, _I64, _I32, _I32, _P]),

@@ -418,6 +418,39 @@ def greedy_argmax(logits: torch.Tensor, out: Optional[torch.Tensor] = None) -> t
     return out
 
 
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor,
+                  top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+                  min_p: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                  logprobs: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """[B, V] logits and uniform numbers u [B] -> [B] int64 token ids, every row with its
+    own temperature, top_k (0: off), top_p (1: off) and min_p (0: off); a temperature of
+    0 gives greedy_argmax's token.  The filters keep a prefix of the tokens ordered by
+    (logit descending, index ascending); the token is the first kept one, in index order,
+    at which the running sum of probabilities exceeds u.  u, temperature, top_p and
+    min_p are fp32 [B], top_k int32 [B]; logprobs (fp32 [B], optional) receives the log
+    of the token's probability among the kept ones.  See as_sample_tokens."""
+    _cuda(logits, u, temperature, top_k, top_p, min_p, out, logprobs)
+    _require(logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1),
+             "sample_tokens: logits must be [B, V] with contiguous rows")
+    B, V = logits.shape
+    for name, t, dt in (("u", u, torch.float32), ("temperature", temperature, torch.float32),
+                        ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                        ("min_p", min_p, torch.float32), ("logprobs", logprobs, torch.float32),
+                        ("out", out, torch.int64)):
+        if t is not None and not (t.dtype == dt and t.shape == (B,) and t.is_contiguous()
+                                  and t.device == logits.device):
+            raise ValueError(f"sample_tokens: {name} must be a contiguous {dt} [B] on the "
+                             "logits' device")
+    if out is None:
+        out = torch.empty(B, dtype=torch.int64, device=logits.device)
+    with torch.cuda.device(logits.device):
+        N.check(N.load().as_sample_tokens(
+            _ptr(out), _ptr(logprobs), _ptr(logits), logits.stride(0) if B > 1 else V, _ptr(u),
+            _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), B, V,
+            dtype_code(logits.dtype), _stream(logits.device)), "as_sample_tokens")
+    return out
+
+
 # ---------------------------------------------------------------------------
 # (5) block gather / copy
 # ---------------------------------------------------------------------------

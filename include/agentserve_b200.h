@@ -29,6 +29,7 @@
  *   as_linear_small_m(_swiglu) nn.Linear of the decode step (llama.py:123-126, 203-211,
  *                             430-431, 471): q/k/v, o_proj, gate/up, down at batch <= 256
  *   as_greedy_argmax          sampling.py:46-58 (greedy branch) + engine.py:379-383
+ *   as_sample_tokens          sampling.py (temperature, top-k, top-p; min-p added)
  *   as_block_copy             cache.py:158-189 (gather_kv) and engine.py:274-281,338-345
  *                             (prefix-cache KV clone / seed)
  *   as_rmsnorm / as_add_rmsnorm / as_silu_mul
@@ -318,6 +319,30 @@ AS_API size_t as_greedy_workspace_size(int32_t num_rows);
 AS_API int as_greedy_argmax(int64_t* out, const void* logits, int64_t row_stride,
                             int32_t num_rows, int32_t vocab, int32_t dtype, void* workspace,
                             size_t workspace_bytes, as_stream_t stream);
+
+/* Sampling of one token per row of logits [num_rows, vocab] from given uniform numbers
+ * (sampling.py's sampled branch, and engine.py:321, 379-383, which sample one request
+ * at a time), every row with its own settings.  With x the sanitised fp32 logits (as
+ * as_greedy_argmax), m their maximum and w = exp((x - m) / temperature), the tokens
+ * are ordered by (x descending, index ascending) and the first
+ * max(1, min(n_k, n_p, n_m)) are kept:
+ *   n_k = top_k (all when top_k <= 0 or >= vocab),
+ *   n_p = the least n whose weights sum to at least top_p times those of the first n_k
+ *         (n_k when top_p >= 1 or NaN),
+ *   n_m = the number of tokens with w >= min_p (all when min_p <= 0 or NaN).
+ * out[r] is the first kept token, in index order, at which the running sum of kept
+ * weights exceeds u[r] times their total; a u outside [0, 1) gives the first or last
+ * kept token of positive weight.  A temperature <= 1e-6 (or NaN) gives
+ * the first maximum, as as_greedy_argmax.  logprobs[r] (NULL to skip) is the log of the
+ * token's weight over the kept total, 0 for a row that keeps one token.
+ * u, temperature, top_p, min_p fp32 and top_k int32 are [num_rows]; top_k, top_p and
+ * min_p may be NULL (off).  Weights are computed in 64 bits and summed in fixed point,
+ * so the result does not depend on the launch; no workspace.  vocab <= 2^24. */
+AS_API int as_sample_tokens(int64_t* out, float* logprobs, const void* logits,
+                            int64_t row_stride, const float* u, const float* temperature,
+                            const int32_t* top_k, const float* top_p, const float* min_p,
+                            int32_t num_rows, int32_t vocab, int32_t dtype,
+                            as_stream_t stream);
 
 /* ------------------------------------------------------------------------- */
 /* (5) Block gather / copy (prefix-cache seeding, gather_kv)                 */

@@ -67,6 +67,13 @@ SIGNATURES = {
                                                 _P]),
     "as_greedy_workspace_size": (_SZ, [_I32]),
     "as_greedy_argmax": (ctypes.c_int, [_P, _P, _I64, _I32, _I32, _I32, _P, _SZ, _P]),
+    "as_shared_prefix_plan_ints": (_I64, [_I32, _I32, _I32, _I32, _I32]),
+    "as_shared_prefix_workspace_size": (_SZ, [_I32, _I32, _I32, _I32, _I32]),
+    "as_shared_prefix_plan": (ctypes.c_int, [_P, _I64, _P, _P, _P, _I32, _P, _I32, _I32, _I32,
+                                             _I32, _I32, _I32]),
+    "as_shared_prefix_decode_attention": (ctypes.c_int, [_P, _P, _I64, _P, _P, _P, _I64, _P, _P,
+                                                         _P, _I32, _I32, _I32, _I32, _I32, _I32,
+                                                         _I32, _F32, _P, _SZ, _I32, _I32, _P]),
     "as_sample_tokens": (ctypes.c_int, [_P, _P, _P, _I64, _P, _P, _P, _P, _P, _I32, _I32, _I32,
                                         _P]),
     "as_rmsnorm": (ctypes.c_int, [_P, _P, _P, _I64, _I32, _F32, _I32, _P]),

@@ -9,8 +9,9 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Sequence
 
+import numpy as np
 import torch
 
 from . import _native as N
@@ -287,6 +288,130 @@ def rope_paged_decode_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
         BLOCK_SIZE, NB, block_tables.shape[1], float(scale), int(blocks_per_split),
         _ptr(workspace), ws_bytes, int(out_layout), dtype_code(q.dtype), _stream(q.device)),
         "as_rope_paged_decode_attention")
+    return out
+
+
+# ---------------------------------------------------------------------------
+# (9) decode attention for a batch that shares leading blocks
+# ---------------------------------------------------------------------------
+class SharedPrefixPlan:
+    """Who shares what in a decode batch, and how its attention is divided over the GPU
+    (shared_prefix_plan).  It stays valid while the same batch rows share the same
+    blocks, whatever their lengths."""
+
+    def __init__(self, num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                 dtype: torch.dtype, device, full_grid: bool):
+        self.num_seqs, self.num_heads, self.num_kv_heads = num_seqs, num_heads, num_kv_heads
+        self.head_dim, self.dtype, self.full_grid = head_dim, dtype, full_grid
+        self.device = torch.device(device)
+        code = dtype_code(dtype)
+        n = int(N.load().as_shared_prefix_plan_ints(num_seqs, num_heads, num_kv_heads, head_dim,
+                                                    code))
+        _require(n > 0, "shared_prefix_plan: needs at least one sequence, heads a multiple of "
+                 "kv_heads and head_dim <= 256")
+        self.workspace_bytes = int(N.load().as_shared_prefix_workspace_size(
+            num_seqs, num_heads, num_kv_heads, head_dim, code))
+        pinned = self.device.type == "cuda"
+        self._host = torch.zeros(n, dtype=torch.int32, pin_memory=pinned)
+        self._header = ctypes.c_void_p(self._host.data_ptr())
+        self.ints = torch.zeros(n, dtype=torch.int32, device=self.device)
+        self._copied = torch.cuda.Event() if pinned else None
+
+    def load(self, groups: Sequence[Sequence[int]], prefix_blocks: Sequence[int],
+             row_blocks: Sequence[int]) -> None:
+        """Replace the plan by another of the same batch size, in the same buffers; with
+        full_grid, launches captured with this plan follow it.  Stream-ordered."""
+        _require(len(groups) == len(prefix_blocks) and len(row_blocks) == self.num_seqs,
+                 "shared_prefix_plan: one prefix_blocks per group and one row_blocks per sequence")
+        offsets = np.zeros(len(groups) + 1, dtype=np.int32)
+        np.cumsum([len(g) for g in groups], out=offsets[1:])
+        members = np.array([b for g in groups for b in g], dtype=np.int32)
+        prefix = np.array(prefix_blocks, dtype=np.int32)
+        rows = np.array(row_blocks, dtype=np.int32)
+        host = np.zeros(self._host.numel(), dtype=np.int32)
+        N.check(N.load().as_shared_prefix_plan(
+            host.ctypes.data, host.size, offsets.ctypes.data, members.ctypes.data,
+            prefix.ctypes.data, len(groups), rows.ctypes.data, self.num_seqs, self.num_heads,
+            self.num_kv_heads, self.head_dim, dtype_code(self.dtype), int(self.full_grid)),
+            "as_shared_prefix_plan")
+        if self._copied is None:
+            self._host.numpy()[:] = host
+            self.ints.copy_(self._host)
+            return
+        with torch.cuda.device(self.device):
+            self._copied.synchronize()  # an earlier copy has left the pinned buffer
+            self._host.numpy()[:] = host
+            self.ints.copy_(self._host, non_blocking=True)
+            self._copied.record()
+
+
+def shared_prefix_plan(groups: Sequence[Sequence[int]], prefix_blocks: Sequence[int],
+                       row_blocks: Sequence[int], num_heads: int, num_kv_heads: int,
+                       head_dim: int, dtype: torch.dtype, device,
+                       full_grid: bool = False) -> SharedPrefixPlan:
+    """groups: lists of batch rows whose block tables start with the same
+    prefix_blocks[i] blocks (rows in no group attend alone); row_blocks [B]: the blocks
+    each row will hold (to balance the work).  full_grid: a launch captured in a CUDA
+    graph with this plan stays right after plan.load() of another one.
+    DeviceBlockAllocator.shared_prefix_groups finds the groups of a batch of requests."""
+    plan = SharedPrefixPlan(len(row_blocks), num_heads, num_kv_heads, head_dim, dtype, device,
+                            full_grid)
+    plan.load(groups, prefix_blocks, row_blocks)
+    return plan
+
+
+def new_shared_prefix_workspace(plan: SharedPrefixPlan) -> torch.Tensor:
+    """Zero-filled workspace of shared_prefix_decode_attention for plans of this batch
+    size and geometry (the kernel keeps its counters at zero between calls)."""
+    return torch.zeros(plan.workspace_bytes, dtype=torch.uint8, device=plan.device)
+
+
+def shared_prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                   block_tables: torch.Tensor, seq_lens_k: torch.Tensor,
+                                   plan: SharedPrefixPlan, scale: float,
+                                   workspace: Optional[torch.Tensor] = None,
+                                   out: Optional[torch.Tensor] = None,
+                                   out_layout: int = N.AS_LAYOUT_HEAD_MAJOR) -> torch.Tensor:
+    """paged_decode_attention for a batch whose groups of sequences share leading blocks
+    (plan): the shared blocks are read and multiplied once per group.  q [B, H, D]
+    (row-strided view allowed, rotated), k_cache/v_cache [NB, 16, Kh, D], block_tables
+    [B, >=max_blocks] int32, seq_lens_k [B] int32 (keys incl. the new token).  Returns
+    out [B, H*D] in out_layout.  workspace: new_shared_prefix_workspace(plan), allocated
+    and cleared per call when not given."""
+    dev = q.device
+    _cuda(q, k_cache, v_cache, block_tables, seq_lens_k, workspace, out)
+    B, H, D = q.shape
+    NB, bs, Kh, D2 = k_cache.shape
+    _require(bs == BLOCK_SIZE and D2 == D and v_cache.shape == k_cache.shape,
+             "k_cache / v_cache must be [NB, 16, Kh, D] with q's head_dim")
+    _require(k_cache.is_contiguous() and v_cache.is_contiguous(), "KV planes must be contiguous")
+    _require(k_cache.dtype == q.dtype and v_cache.dtype == q.dtype,
+             "k_cache / v_cache must have q's dtype")
+    _require(_row_view_ok(q) and (B == 1 or q.stride(0) >= H * D),
+             "q must be [B, H, D] with contiguous rows")
+    _require(block_tables.dtype == torch.int32 and block_tables.dim() == 2 and
+             block_tables.shape[0] == B and block_tables.shape[1] > 0 and
+             (block_tables.stride(1) == 1 or block_tables.shape[1] == 1),
+             "block_tables must be int32 [B, max_blocks] with contiguous rows")
+    _require(seq_lens_k.dtype == torch.int32 and seq_lens_k.shape == (B,) and
+             seq_lens_k.is_contiguous(), "seq_lens_k must be a contiguous int32 [B]")
+    _require(plan.dtype == q.dtype and plan.num_seqs == B, "the plan was made for another batch")
+    for t in (k_cache, v_cache, block_tables, seq_lens_k, plan.ints, workspace, out):
+        _require(t is None or t.device == dev, "all tensors must be on q's device")
+    if out is None:
+        out = torch.empty(B, H * D, dtype=q.dtype, device=dev)
+    _require(out.shape == (B, H * D) and out.dtype == q.dtype and out.is_contiguous(),
+             "out must be a contiguous [B, H*D] of q's dtype")
+    if workspace is None:
+        workspace = new_shared_prefix_workspace(plan)
+    bt_stride = block_tables.stride(0) if B > 1 else block_tables.shape[1]
+    with torch.cuda.device(dev):
+        N.check(N.load().as_shared_prefix_decode_attention(
+            _ptr(out), _ptr(q), q.stride(0) if B > 1 else H * D, _ptr(k_cache), _ptr(v_cache),
+            _ptr(block_tables), bt_stride, _ptr(seq_lens_k), plan._header, _ptr(plan.ints), B, H,
+            Kh, D, BLOCK_SIZE, NB, block_tables.shape[1], float(scale), _ptr(workspace),
+            workspace.numel() * workspace.element_size(), int(out_layout), dtype_code(q.dtype),
+            _stream(dev)), "as_shared_prefix_decode_attention")
     return out
 
 

@@ -24,6 +24,8 @@
  *                             and llama.py:303-361 (padded-list decode)
  *   as_rope_paged_decode_attention  llama.py:433-469 (RoPE of the new token, its
  *                             write_kv_decode and the attention) in one launch
+ *   as_shared_prefix_decode_attention  the same, for sequences whose leading blocks are
+ *                             the same ones (prefix-cache hits, engine.py:274-281)
  *   as_varlen_prefill_attention llama.py:128-186 (prefill over cached prefix + new tokens)
  *   as_varlen_prefill_attention_ws  the same, split-KV over CTAs with a workspace
  *   as_linear_small_m(_swiglu) nn.Linear of the decode step (llama.py:123-126, 203-211,
@@ -229,6 +231,54 @@ AS_API int as_paged_decode_attention_noalloc(void* out, const void* q, int64_t q
                                              int32_t num_blocks, int32_t max_blocks, float scale,
                                              int32_t blocks_per_split, int32_t out_layout,
                                              int32_t dtype, as_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* (9) Decode attention for a batch that shares leading blocks               */
+/* ------------------------------------------------------------------------- */
+
+/* The attention of as_paged_decode_attention for a batch in which groups of sequences
+ * hold the same leading blocks (a prefix-cache hit shares them; the reference clones
+ * the prefix per request, engine.py:274-281, and attends over every copy,
+ * llama.py:419-469): a group's shared blocks are read and multiplied once for all its
+ * members.  Results equal as_paged_decode_attention's up to rounding.
+ *
+ * as_shared_prefix_plan divides the work, on the host: group i of num_groups is the
+ * batch rows members[group_offsets[i] .. group_offsets[i+1]-1] whose block tables start
+ * with the same prefix_blocks[i] blocks; no row may be in two groups, and rows in none
+ * attend alone.  row_blocks[b] is the number of blocks row b will hold (at least its
+ * group's prefix_blocks; used to balance the work, the lengths themselves are read on
+ * the device at every call).  The plan stays valid while the same rows share the same
+ * blocks.  plan: as_shared_prefix_plan_ints() ints of host memory (`capacity` of them
+ * available).  The caller copies all of them to the device, and passes both: the
+ * device copy, and the host copy's first AS_SHARED_PREFIX_HEADER ints, which size the
+ * launch.  full_grid != 0 sizes it for any plan of the same batch size and geometry,
+ * so that a captured launch may be replayed after another plan was copied over the
+ * device buffer; 0 sizes it for this plan.  A plan with no group is valid.
+ *
+ * The attention itself: seq_lens_k counts the new token, whose K/V must be in the pool.
+ * A row shorter than its group's shared blocks is attended alone (correct, not shared);
+ * a row of length 0 gives zeros.  workspace: as_shared_prefix_workspace_size() bytes,
+ * 256-byte aligned, zero before its first call; each call leaves it fit for the next
+ * of the same num_seqs and geometry.  Calls sharing a workspace must be
+ * stream-ordered.  num_seqs <= 65535, head_dim <= 256. */
+#define AS_SHARED_PREFIX_HEADER 32
+AS_API int64_t as_shared_prefix_plan_ints(int32_t num_seqs, int32_t num_heads,
+                                          int32_t num_kv_heads, int32_t head_dim, int32_t dtype);
+AS_API size_t as_shared_prefix_workspace_size(int32_t num_seqs, int32_t num_heads,
+                                              int32_t num_kv_heads, int32_t head_dim,
+                                              int32_t dtype);
+AS_API int as_shared_prefix_plan(int32_t* plan, int64_t capacity, const int32_t* group_offsets,
+                                 const int32_t* members, const int32_t* prefix_blocks,
+                                 int32_t num_groups, const int32_t* row_blocks, int32_t num_seqs,
+                                 int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                 int32_t dtype, int32_t full_grid);
+AS_API int as_shared_prefix_decode_attention(
+    void* out, const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
+    const int32_t* block_tables, int64_t bt_stride, const int32_t* seq_lens_k,
+    const int32_t* plan_header, const int32_t* plan, int32_t num_seqs, int32_t num_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t num_blocks,
+    int32_t max_blocks, float scale, void* workspace, size_t workspace_bytes, int32_t out_layout,
+    int32_t dtype, as_stream_t stream);
 
 /* ------------------------------------------------------------------------- */
 /* (4) Varlen prefill attention over cached prefix blocks + new tokens       */

@@ -30,6 +30,7 @@ AS_DECODE_NOALLOC_SCRATCH_BYTES = 8 << 20
 
 AS_KERNEL_DECODE_ATTENTION = 1
 AS_KERNEL_PREFILL_ATTENTION = 2
+AS_KERNEL_SHARED_PREFIX = 4
 
 # Every exported entry point with its C signature (restype, argtypes).
 _P = ctypes.c_void_p

@@ -147,7 +147,8 @@ extern "C" uint64_t as_set_wait_limit_ns(uint64_t limit_ns) {
 }
 
 extern "C" int as_debug_starve_next_launch(int kernels) {
-  if (kernels & ~(AS_KERNEL_DECODE_ATTENTION | AS_KERNEL_PREFILL_ATTENTION))
+  if (kernels & ~(AS_KERNEL_DECODE_ATTENTION | AS_KERNEL_PREFILL_ATTENTION |
+                  AS_KERNEL_SHARED_PREFIX))
     return asb::fail(AS_ERR_INVALID_ARG, "as_debug_starve_next_launch: unknown kernel bits %d",
                      kernels);
   asb::g_starve_next.store(kernels);

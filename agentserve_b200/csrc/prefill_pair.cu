@@ -31,6 +31,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "f32x2.cuh"
 #include "host_util.h"
 #include "prefill_tcgen05.h"
 #include "tcgen05.cuh"
@@ -61,25 +62,6 @@ int pair_count(int max_seqlen_q, int H, int Kh) {
 #ifndef AS_PREFILL_HANDOFF
 #define AS_PREFILL_HANDOFF 32
 #endif
-// ---- packed fp32 pairs (sm_100 f32x2 arithmetic) --------------------------------
-__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 // 2^x for a pair of fp32 values on the FMA pipe instead of the exponent unit (the
 // softmax at head_dim 64 is bound by the exponent unit: 16 results per clock per SM).
 // Cody-Waite style split x = j + f with j = floor(x), f in [0, 1): adding 1.5 * 2^23
@@ -120,12 +102,6 @@ __device__ __forceinline__ uint64_t exp2_poly_f2(uint64_t x2) {
   return f2_pack(ea, eb);
 }
 #endif
-
-__device__ __forceinline__ float max3f(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
 
 // Keys per KV tile at head_dim 128: 128 (default) or 64.  With 128, S (128 columns)
 // and O (128) fill a query tile's 256 TMEM columns, so P must alias S and S(j+1) can

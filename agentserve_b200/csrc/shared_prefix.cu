@@ -42,7 +42,8 @@ struct GenCfg {
   static constexpr int kTokens = 32 * TG;
   static constexpr int kLdK = DP + 4;  // float4 reads of 8 lanes hit 32 different banks
   static constexpr int kFloats = kRows * DP + kTokens * kLdK + kTokens * DP + kNWarps * RW * 32;
-  static constexpr int kMerge = TG * kRows * (DP + 2);  // reuses the K / V space
+  static constexpr int kJoin = TG * kRows * (DP + 2);  // reuses the K / V space
+  static constexpr int kMerge = kJoin + join_scratch(kRows, kThreads);
   static constexpr int kSmemBytes = 4 * (kFloats > kMerge ? kFloats : kMerge);
 };
 
@@ -72,8 +73,9 @@ sp_generic_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
   if (kPrefix) {
     const int32_t* it = plan + plan[kHOffPrefix] + blockIdx.x * kPrefixInts;
     members = plan + plan[kHOffMembers] + it[kPMembers];
-    row0 = it[kPRow0];
-    rows = it[kPRows];
+    row0 = it[kPRow0] + blockIdx.z * Cfg::kRows;  // the plan's tiles may be larger
+    rows = min(Cfg::kRows, it[kPRows] - int(blockIdx.z) * Cfg::kRows);
+    if (rows <= 0) return;
     begin = it[kPBegin] * kBS;
     end = it[kPEnd] * kBS;
     part = it[kPPart];
@@ -256,47 +258,49 @@ sp_generic_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
     }
     return;
   }
-  finish_own<T, false>(a, rp, out, b, split, g * group + row0, rows, ro, DP, rm, rl);
+  finish_own<T, false, Cfg::kRows, kThreads>(a, rp, out, b, split, g * group + row0, rows, ro, DP,
+                                             rm, rl, smem + Cfg::kJoin);
   pdl_wait();  // this launch ends after the prefix launch before it
 }
 
 constexpr int kGenericRows = 32;
 
 template <typename T, int DP, int RW, int TG, bool kPrefix>
-int launch_generic_one(dim3 grid, T* out, const T* q, const T* k, const T* v, const Args& a,
+int launch_generic_one(dim3 grid, int tile_rows, T* out, const T* q, const T* k, const T* v, const Args& a,
                        cudaStream_t s) {
   using Cfg = GenCfg<DP, RW, TG>;
   auto kern = sp_generic_kernel<T, DP, RW, TG, kPrefix>;
   if (Cfg::kSmemBytes > 48 * 1024)
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
-  grid.z = kPrefix ? 1 : (a.group + Cfg::kRows - 1) / Cfg::kRows;
+  grid.z = kPrefix ? (tile_rows + Cfg::kRows - 1) / Cfg::kRows
+                   : (a.group + Cfg::kRows - 1) / Cfg::kRows;
   launch_pdl(kern, grid, dim3(kThreads), Cfg::kSmemBytes, s, out, q, k, v, a);
   return check_launch("as_shared_prefix_decode_attention");
 }
 
 template <typename T, int DP>
-int launch_generic(int prefix_grid, int own_grid, T* out, const T* q, const T* k, const T* v,
+int launch_generic(int prefix_grid, int own_grid, int tile_rows, T* out, const T* q, const T* k, const T* v,
                    const Args& a, cudaStream_t s) {
   if (prefix_grid > 0) {
-    const int rc = launch_generic_one<T, DP, 4, 1, true>(dim3(prefix_grid, a.Kh), out, q, k, v,
-                                                         a, s);
+    const int rc = launch_generic_one<T, DP, 4, 1, true>(dim3(prefix_grid, a.Kh), tile_rows, out,
+                                                         q, k, v, a, s);
     if (rc) return rc;
   }
   const dim3 grid(own_grid, a.Kh);
   // few heads per KV head: warps share the tokens instead
   if (a.group <= 4 && DP <= 128)
-    return launch_generic_one<T, DP, 1, 2, false>(grid, out, q, k, v, a, s);
-  if (a.group <= 8) return launch_generic_one<T, DP, 1, 1, false>(grid, out, q, k, v, a, s);
-  return launch_generic_one<T, DP, 4, 1, false>(grid, out, q, k, v, a, s);
+    return launch_generic_one<T, DP, 1, 2, false>(grid, tile_rows, out, q, k, v, a, s);
+  if (a.group <= 8) return launch_generic_one<T, DP, 1, 1, false>(grid, tile_rows, out, q, k, v, a, s);
+  return launch_generic_one<T, DP, 4, 1, false>(grid, tile_rows, out, q, k, v, a, s);
 }
 
 template <typename T>
-int launch_generic_dim(int prefix_grid, int own_grid, T* out, const T* q, const T* k, const T* v,
+int launch_generic_dim(int prefix_grid, int own_grid, int tile_rows, T* out, const T* q, const T* k, const T* v,
                        const Args& a, cudaStream_t s) {
-  if (a.D <= 32) return launch_generic<T, 32>(prefix_grid, own_grid, out, q, k, v, a, s);
-  if (a.D <= 64) return launch_generic<T, 64>(prefix_grid, own_grid, out, q, k, v, a, s);
-  if (a.D <= 128) return launch_generic<T, 128>(prefix_grid, own_grid, out, q, k, v, a, s);
-  return launch_generic<T, 256>(prefix_grid, own_grid, out, q, k, v, a, s);
+  if (a.D <= 32) return launch_generic<T, 32>(prefix_grid, own_grid, tile_rows, out, q, k, v, a, s);
+  if (a.D <= 64) return launch_generic<T, 64>(prefix_grid, own_grid, tile_rows, out, q, k, v, a, s);
+  if (a.D <= 128) return launch_generic<T, 128>(prefix_grid, own_grid, tile_rows, out, q, k, v, a, s);
+  return launch_generic<T, 256>(prefix_grid, own_grid, tile_rows, out, q, k, v, a, s);
 }
 
 // ===========================================================================
@@ -317,7 +321,7 @@ struct Limits {
 Limits limits(int B, int H, int Kh, int D, int dtype) {
   Limits n{};
   const int group = H / Kh;
-  n.tile_rows = kGenericRows;
+  n.tile_rows = tc_geometry(D, dtype) ? kTcTileRows : kGenericRows;
   n.prefix_slots = 2 * sm_count();
   n.own_slots = 6 * sm_count();
   n.min_prefix = 8;
@@ -327,8 +331,6 @@ Limits limits(int B, int H, int Kh, int D, int dtype) {
   n.own_items = (n.own_slots + Kh - 1) / Kh + B;
   n.prefix_parts = B + (int64_t(n.prefix_slots) * n.tile_rows + H - 1) / H;
   n.own_parts = n.own_items;
-  (void)D;
-  (void)dtype;
   return n;
 }
 
@@ -338,7 +340,7 @@ int64_t plan_ints(const Limits& n, int B) {
 }
 
 bool sizes_ok(int B, int H, int Kh, int D, int dtype) {
-  return B > 0 && B <= 65535 && H > 0 && Kh > 0 && H % Kh == 0 && Kh <= 65535 && D > 0 &&
+  return B > 0 && B <= 65535 && H > 0 && Kh > 0 && H % Kh == 0 && H <= 65535 && D > 0 &&
          D <= 256 && dtype_size(dtype) > 0 && int64_t(B) * H < (int64_t(1) << 30);
 }
 
@@ -428,7 +430,7 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
     for (;; chunk += chunk / 2) {
       int64_t parts = 0;
       for (Group& g : groups) {
-        g.splits = int((g.blocks + chunk - 1) / chunk);
+        g.splits = int(std::min<int64_t>(kMaxSplits, (g.blocks + chunk - 1) / chunk));
         g.chunk = (g.blocks + g.splits - 1) / g.splits;
         g.splits = (g.blocks + g.chunk - 1) / g.chunk;
         parts += int64_t(g.splits) * g.size;
@@ -481,7 +483,7 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
     int64_t own_part = 0;
     for (int b = 0; b < B; ++b) {
       const int blocks = row_blocks[b] - shared[b];
-      const int splits = std::max<int>(1, int((blocks + own_chunk - 1) / own_chunk));
+      const int splits = std::clamp<int>(int((blocks + own_chunk - 1) / own_chunk), 1, kMaxSplits);
       int32_t* r = rows + int64_t(b) * kRowInts;
       r[kROwnSplits] = splits;
       r[kROwnPart] = int32_t(own_part);
@@ -539,6 +541,8 @@ extern "C" int as_shared_prefix_decode_attention(
                 num_seqs, num_heads, num_kv_heads, head_dim, num_blocks, max_blocks);
   if (out_layout != AS_LAYOUT_HEAD_MAJOR && out_layout != AS_LAYOUT_DIM_MAJOR)
     return fail(AS_ERR_INVALID_ARG, "%s: unknown out_layout %d", who, out_layout);
+  if (!(scale > 0.f) || scale > 3e38f)
+    return fail(AS_ERR_INVALID_ARG, "%s: scale must be positive and finite", who);
   if (!out || !q || !k_cache || !v_cache || !block_tables || !seq_lens_k || !plan_header || !plan)
     return fail(AS_ERR_INVALID_ARG, "%s: null pointer", who);
   const int32_t* h = plan_header;
@@ -585,9 +589,14 @@ extern "C" int as_shared_prefix_decode_attention(
   a.status = device_status_ptr();
   a.wait_limit = wait_limit_ns();
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  // TMA reads the planes from 16-byte boundaries; others take the CUDA-core kernels
+  const bool aligned = ((reinterpret_cast<uintptr_t>(k_cache) |
+                         reinterpret_cast<uintptr_t>(v_cache)) & 15) == 0;
+  if (tc_geometry(head_dim, dtype) && aligned)
+    return tc_launch(h[kHPrefixGrid], h[kHOwnGrid], out, q, k_cache, v_cache, a, dtype, s);
   auto run = [&](auto tag) -> int {
     using T = decltype(tag);
-    return launch_generic_dim<T>(h[kHPrefixGrid], h[kHOwnGrid], static_cast<T*>(out),
+    return launch_generic_dim<T>(h[kHPrefixGrid], h[kHOwnGrid], n.tile_rows, static_cast<T*>(out),
                                  static_cast<const T*>(q), static_cast<const T*>(k_cache),
                                  static_cast<const T*>(v_cache), a, s);
   };

@@ -95,18 +95,31 @@ __device__ __forceinline__ float part_exp(float x) {
   return kBase2 ? fast_exp2(x) : expf(x);
 }
 
-// Ends an own item: rows [h0, h0 + nr) of sequence b, whose part of split s is in shared
-// memory (o [nr][ld], m, l).  Joins it with the other parts of the row when it is the
-// last to arrive, and writes the output.  All threads of the block call this.
-template <typename T, bool kBase2>
+// Most parts a row has of either kind (the plan keeps to it), so that the weights of a
+// join fit in shared memory.
+constexpr int kMaxSplits = 64;
+
+// Shared-memory floats a join works in.
+constexpr int join_scratch(int rows, int threads) { return rows * 2 * kMaxSplits + 4 * threads; }
+
+// Ends an own item: rows [h0, h0 + nr) of sequence b, nr <= kRows, whose part of split
+// `split` is in shared memory (o [nr][ld], m, l).  Joins it with the other parts of the
+// rows when it is the last to arrive, and writes the output.  All threads of the block
+// call this.  A warp per row turns the parts' (m, l) into weights; then every thread
+// sums its share of the parts for four dimensions of a row, so the loads of the parts,
+// which come from L2, are all in flight at once.  scratch: join_scratch() floats of
+// shared memory, apart from o, m and l.
+template <typename T, bool kBase2, int kRows, int kThreads>
 __device__ void finish_own(const Args& a, const RowPlan& p, T* __restrict__ out, int b, int split,
                            int h0, int nr, const float* o, int ld, const float* m,
-                           const float* l) {
+                           const float* l, float* scratch) {
   __shared__ int s_last;
+  auto s_w = reinterpret_cast<float(*)[2 * kMaxSplits]>(scratch + 4 * kThreads);
+  float4* s_sum = reinterpret_cast<float4*>(scratch);  // 16-byte aligned
   const int D = a.D, H = a.H;
   const bool alone = p.own_splits == 1;
   if (!alone) {
-    for (int i = threadIdx.x; i < nr * D; i += blockDim.x) {
+    for (int i = threadIdx.x; i < nr * D; i += kThreads) {
       const int r = i / D, d = i - r * D;
       const size_t at = size_t(p.own_part + split) * H + h0 + r;
       a.parts.o[at * D + d] = o[r * ld + d];
@@ -122,44 +135,109 @@ __device__ void finish_own(const Args& a, const RowPlan& p, T* __restrict__ out,
     }
     __syncthreads();
     if (!s_last) return;
+    if (threadIdx.x == 0) a.parts.counters[b * H + h0] = 0;  // for the next call
   }
   if (p.prefix_splits > 0 && !a.wait_first) pdl_wait();  // the prefix parts are written
-  for (int i = threadIdx.x; i < nr * D; i += blockDim.x) {
-    const int r = i / D, d = i - r * D, h = h0 + r;
-    float M = alone ? m[r] : -INFINITY;
-    if (!alone)
-      for (int s = 0; s < p.own_splits; ++s)
-        M = fmaxf(M, __ldcg(&a.parts.ml[size_t(p.own_part + s) * H + h]).x);
-    for (int s = 0; s < p.prefix_splits; ++s)
-      M = fmaxf(M, __ldcg(&a.parts.ml[(size_t(p.prefix_part) + size_t(s) * p.prefix_step) * H + h]).x);
-    float L = 0.f, O = 0.f;
-    if (M != -INFINITY) {
-      if (alone) {
-        const float w = part_exp<kBase2>(m[r] - M);
-        L = w * l[r];
-        O = w * o[r * ld + d];
-      } else {
-        for (int s = 0; s < p.own_splits; ++s) {
-          const size_t at = size_t(p.own_part + s) * H + h;
-          const float2 ml = __ldcg(&a.parts.ml[at]);
-          const float w = part_exp<kBase2>(ml.x - M);
-          L += w * ml.y;
-          O += w * __ldcg(&a.parts.o[at * D + d]);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int np = p.prefix_splits + (alone ? 1 : p.own_splits);
+  const auto part = [&](int s) -> size_t {
+    return s < p.prefix_splits ? size_t(p.prefix_part) + size_t(s) * p.prefix_step
+                               : size_t(p.own_part + s - p.prefix_splits);
+  };
+  for (int r = warp; r < nr; r += kThreads / 32) {
+    float2 ml[2 * kMaxSplits / 32];
+    float M = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2 * kMaxSplits / 32; ++i) {
+      const int s = lane + 32 * i;
+      ml[i] = make_float2(-INFINITY, 0.f);
+      if (s < np)
+        ml[i] = alone && s == np - 1 ? make_float2(m[r], l[r])
+                                     : __ldcg(&a.parts.ml[part(s) * H + h0 + r]);
+      M = fmaxf(M, ml[i].x);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    float L = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2 * kMaxSplits / 32; ++i) {
+      ml[i].x = ml[i].x == -INFINITY ? 0.f : part_exp<kBase2>(ml[i].x - M);
+      L += ml[i].x * ml[i].y;
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);  // NaN stays NaN
+#pragma unroll
+    for (int i = 0; i < 2 * kMaxSplits / 32; ++i)
+      if (lane + 32 * i < np) s_w[r][lane + 32 * i] = ml[i].x * inv;
+  }
+  __syncthreads();
+  if ((D & 3) == 0) {
+    const int nv = nr * (D / 4);
+    for (int v0 = 0; v0 < nv; v0 += kThreads) {
+      // as many threads as there are vectors share out the parts
+      const int here = min(nv - v0, kThreads), ways = kThreads / here;
+      const int v = v0 + threadIdx.x % here, way = threadIdx.x / here;
+      const int r = v / (D / 4), d = (v - r * (D / 4)) * 4;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (way < ways) {
+#pragma unroll 4
+        for (int s = way; s < np; s += ways) {
+          const float w = s_w[r][s];
+          if (w == 0.f) continue;  // a part without keys holds no values
+          const float4 x =
+              alone && s == np - 1
+                  ? make_float4(o[r * ld + d], o[r * ld + d + 1], o[r * ld + d + 2],
+                                o[r * ld + d + 3])
+                  : __ldcg(reinterpret_cast<const float4*>(
+                        &a.parts.o[(part(s) * H + h0 + r) * D + d]));
+          acc.x += w * x.x;
+          acc.y += w * x.y;
+          acc.z += w * x.z;
+          acc.w += w * x.w;
         }
       }
-      for (int s = 0; s < p.prefix_splits; ++s) {
-        const size_t at = (size_t(p.prefix_part) + size_t(s) * p.prefix_step) * H + h;
-        const float2 ml = __ldcg(&a.parts.ml[at]);
-        const float w = part_exp<kBase2>(ml.x - M);
-        L += w * ml.y;
-        O += w * __ldcg(&a.parts.o[at * D + d]);
+      s_sum[threadIdx.x] = acc;
+      __syncthreads();
+      if (threadIdx.x < here) {
+        for (int y = 1; y < ways; ++y) {
+          const float4 x = s_sum[threadIdx.x + y * here];
+          acc.x += x.x;
+          acc.y += x.y;
+          acc.z += x.z;
+          acc.w += x.w;
+        }
+        T* dst = out + size_t(b) * H * D + size_t(h0 + r) * a.os_h + size_t(d) * a.os_d;
+        dst[0] = Elem<T>::from_f32(acc.x);
+        dst[a.os_d] = Elem<T>::from_f32(acc.y);
+        dst[2 * size_t(a.os_d)] = Elem<T>::from_f32(acc.z);
+        dst[3 * size_t(a.os_d)] = Elem<T>::from_f32(acc.w);
       }
+      __syncthreads();
     }
-    out[size_t(b) * H * D + size_t(h) * a.os_h + size_t(d) * a.os_d] =
-        Elem<T>::from_f32(L > 0.f ? O / L : 0.f);
+    return;
   }
-  if (!alone && threadIdx.x == 0) a.parts.counters[b * H + h0] = 0;  // for the next call
+  for (int i = threadIdx.x; i < nr * D; i += kThreads) {
+    const int r = i / D, d = i - r * D;
+    float acc = 0.f;
+    for (int s = 0; s < np; ++s) {
+      const float w = s_w[r][s];
+      if (w == 0.f) continue;
+      acc += w * (alone && s == np - 1 ? o[r * ld + d]
+                                       : __ldcg(&a.parts.o[(part(s) * H + h0 + r) * D + d]));
+    }
+    out[size_t(b) * H * D + size_t(h0 + r) * a.os_h + size_t(d) * a.os_d] =
+        Elem<T>::from_f32(acc);
+  }
 }
+
+// Tensor-core launches (shared_prefix_tc.cu): 16-bit types, head_dim 64 or 128.
+constexpr int kTcTileRows = 128;
+inline bool tc_geometry(int D, int dtype) {
+  return (dtype == AS_DTYPE_BF16 || dtype == AS_DTYPE_F16) && (D == 64 || D == 128);
+}
+int tc_launch(int prefix_grid, int own_grid, void* out, const void* q, const void* k_cache,
+              const void* v_cache, const Args& a, int dtype, cudaStream_t stream);
 
 }  // namespace sp
 }  // namespace asb

@@ -98,6 +98,8 @@ AS_API uint64_t as_set_wait_limit_ns(uint64_t limit_ns);
  * Each call replaces the pending set (0 clears it). */
 #define AS_KERNEL_DECODE_ATTENTION 1  /* as_paged_decode_attention, bf16/fp16 fast path */
 #define AS_KERNEL_PREFILL_ATTENTION 2 /* as_varlen_prefill_attention*, tcgen05 path */
+#define AS_KERNEL_SHARED_PREFIX 4     /* as_shared_prefix_decode_attention, tensor-core path:
+                                         both its launches */
 AS_API int as_debug_starve_next_launch(int kernels);
 
 /* ------------------------------------------------------------------------- */
@@ -260,7 +262,7 @@ AS_API int as_paged_decode_attention_noalloc(void* out, const void* q, int64_t q
  * a row of length 0 gives zeros.  workspace: as_shared_prefix_workspace_size() bytes,
  * 256-byte aligned, zero before its first call; each call leaves it fit for the next
  * of the same num_seqs and geometry.  Calls sharing a workspace must be
- * stream-ordered.  num_seqs <= 65535, head_dim <= 256. */
+ * stream-ordered.  num_seqs <= 65535, head_dim <= 256, scale > 0. */
 #define AS_SHARED_PREFIX_HEADER 32
 AS_API int64_t as_shared_prefix_plan_ints(int32_t num_seqs, int32_t num_heads,
                                           int32_t num_kv_heads, int32_t head_dim, int32_t dtype);

@@ -151,14 +151,16 @@ def test_attention_checks_its_arguments_first(lib):
     head = p._host.data_ptr()
 
     def call(B=4, H=32, Kh=8, D=64, bs=16, NB=100, mb=10, stride=10, qs=2048, ptr=256, ws=256,
-             n=1 << 40, layout=0, dtype=N.AS_DTYPE_BF16, header=head):
+             n=1 << 40, scale=0.125, layout=0, dtype=N.AS_DTYPE_BF16, header=head):
         return lib.as_shared_prefix_decode_attention(
-            ptr, ptr, qs, ptr, ptr, ptr, stride, ptr, header, ptr, B, H, Kh, D, bs, NB, mb, 0.125,
+            ptr, ptr, qs, ptr, ptr, ptr, stride, ptr, header, ptr, B, H, Kh, D, bs, NB, mb, scale,
             ws, n, layout, dtype, None)
     assert call(dtype=7) == N.AS_ERR_INVALID_ARG and "dtype" in N.last_error()
     assert call(bs=8) == N.AS_ERR_UNSUPPORTED and "block_size" in N.last_error()
     for bad in (dict(B=-1), dict(Kh=5), dict(NB=0), dict(mb=0), dict(stride=9), dict(qs=2047)):
         assert call(**bad) == N.AS_ERR_INVALID_ARG and "bad sizes" in N.last_error()
+    for bad in (0.0, -0.5, float("nan"), float("inf")):
+        assert call(scale=bad) == N.AS_ERR_INVALID_ARG and "scale" in N.last_error()
     assert call(layout=2) == N.AS_ERR_INVALID_ARG and "out_layout" in N.last_error()
     assert call(ptr=None) == N.AS_ERR_INVALID_ARG and "null pointer" in N.last_error()
     for bad in (dict(B=3), dict(H=16, qs=2048), dict(D=32), dict(dtype=N.AS_DTYPE_F16)):

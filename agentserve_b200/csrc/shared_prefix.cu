@@ -13,6 +13,7 @@
 // A host-side plan divides both kinds of work over the GPU.  It holds for as long as the
 // same sequences share the same blocks: lengths are read on the device at every call.
 #include <algorithm>
+#include <utility>
 #include <vector>
 
 #include "common.cuh"
@@ -57,41 +58,38 @@ sp_generic_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
     pdl_wait();
     pdl_trigger();
   }
-  const int32_t* plan = a.plan;
-  if (int(blockIdx.x) >= plan[kPrefix ? kHPrefixItems : kHOwnItems]) {
-    if (!kPrefix) pdl_wait();
-    return;
-  }
   const int g = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int D = a.D, group = a.group;
 
   // this item's query rows and token range
-  int b = 0, split = 0, row0 = 0, rows = 0, begin, end, part = 0, table_row;
+  int b = 0, split = 0, row0, rows, begin, end, part = 0, step = 0, table_row;
   const int32_t* members = nullptr;
   RowPlan rp{};
   if (kPrefix) {
-    const int32_t* it = plan + plan[kHOffPrefix] + blockIdx.x * kPrefixInts;
-    members = plan + plan[kHOffMembers] + it[kPMembers];
-    row0 = it[kPRow0] + blockIdx.z * Cfg::kRows;  // the plan's tiles may be larger
-    rows = min(Cfg::kRows, it[kPRows] - int(blockIdx.z) * Cfg::kRows);
+    const PrefixItem it = load_item(a.prefix_items, blockIdx.x);
+    members = a.members + it.members;
+    row0 = it.row0 + blockIdx.z * Cfg::kRows;  // the plan's tiles may be larger
+    rows = min(Cfg::kRows, it.rows - int(blockIdx.z) * Cfg::kRows);
     if (rows <= 0) return;
-    begin = it[kPBegin] * kBS;
-    end = it[kPEnd] * kBS;
-    part = it[kPPart];
-    table_row = members[0];
+    begin = it.begin * kBS;
+    end = it.end * kBS;
+    part = it.part;
+    step = it.step;
+    table_row = it.table_row;
   } else {
-    const int32_t* it = plan + plan[kHOffOwn] + blockIdx.x * kOwnInts;
-    b = it[kORow];
-    split = it[kOSplit];
+    const OwnItem it = load_item(a.own_items, blockIdx.x);
+    if (it.own_splits == 0) {
+      pdl_wait();
+      return;
+    }
+    b = table_row = it.row;
+    split = it.split;
     row0 = blockIdx.z * Cfg::kRows;
     rows = min(Cfg::kRows, group - row0);
-    rp = row_plan(a, b, threadIdx.x == 0 && split == 0 && g == 0 && row0 == 0);
-    const int own = rp.blocks - rp.shared;
-    const int per = (own + rp.own_splits - 1) / rp.own_splits;
-    begin = (rp.shared + min(own, split * per)) * kBS;
-    end = min(rp.len, (rp.shared + min(own, (split + 1) * per)) * kBS);
-    table_row = b;
+    rp = row_plan(a, it, threadIdx.x == 0 && split == 0 && g == 0 && row0 == 0);
+    begin = rp.begin * kBS;
+    end = min(rp.len, (rp.begin + rp.count) * kBS);
   }
 
   extern __shared__ __align__(16) float smem[];
@@ -254,7 +252,11 @@ sp_generic_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
       const int r = i / D, d = i - r * D, rr = row0 + r;
       const size_t at = size_t(part + rr / group) * a.H + g * group + rr % group;
       a.parts.o[at * D + d] = ro[r * DP + d];
-      if (d == 0) a.parts.ml[at] = make_float2(rm[r], rl[r]);
+      if (d == 0) {
+        a.parts.ml[at] = make_float2(rm[r], rl[r]);
+        // one part holds both halves of the keys here
+        if (step > 0) a.parts.ml[at + size_t(step) * a.H] = make_float2(-INFINITY, 0.f);
+      }
     }
     return;
   }
@@ -264,6 +266,10 @@ sp_generic_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
 }
 
 constexpr int kGenericRows = 32;
+// Fixed costs of a block, in the units of its piece: 128-key softmax passes, and blocks.
+constexpr int64_t kPrefixOverhead = 5;
+constexpr int64_t kOwnOverhead = 16;
+constexpr int64_t kMinOwn = 8;  // blocks: two per consumer warp
 
 template <typename T, int DP, int RW, int TG, bool kPrefix>
 int launch_generic_one(dim3 grid, int tile_rows, T* out, const T* q, const T* k, const T* v, const Args& a,
@@ -309,34 +315,61 @@ int launch_generic_dim(int prefix_grid, int own_grid, int tile_rows, T* out, con
 // Sizes that depend on the batch size and the geometry alone, so a captured graph and
 // its workspace serve every plan of the same batch size.
 struct Limits {
-  int tile_rows;      // query rows of a prefix item
-  int prefix_slots;   // prefix blocks (CTAs) aimed at, over all KV heads
-  int own_slots;      // own CTAs aimed at
-  int min_prefix;     // smallest prefix split, in 16-token blocks
-  int min_own;
-  int prefix_items, own_items;    // most items a plan can have
+  bool tc;
+  int tile_rows;     // most query rows of a prefix item
+  int prefix_slots;  // prefix blocks (CTAs) that run at once, over all KV heads
+  int own_slots;     // own CTAs that run at once
+  int own_per_item;  // CTAs of an own item
+  int prefix_items, own_items;      // most items a plan can have
   int64_t prefix_parts, own_parts;  // most parts (of H heads each)
 };
 
 Limits limits(int B, int H, int Kh, int D, int dtype) {
   Limits n{};
   const int group = H / Kh;
-  n.tile_rows = tc_geometry(D, dtype) ? kTcTileRows : kGenericRows;
-  n.prefix_slots = 2 * sm_count();
-  n.own_slots = 6 * sm_count();
-  n.min_prefix = 8;
-  n.min_own = 8;
-  const int tiles = (int(int64_t(B) * group / n.tile_rows) + B / 2 + 1);
-  n.prefix_items = (n.prefix_slots + Kh - 1) / Kh + tiles;
-  n.own_items = (n.own_slots + Kh - 1) / Kh + B;
-  n.prefix_parts = B + (int64_t(n.prefix_slots) * n.tile_rows + H - 1) / H;
+  n.tc = tc_geometry(D, dtype);
+  n.tile_rows = n.tc ? kTcTileRows : kGenericRows;
+  n.prefix_slots = (n.tc ? 1 : 2) * sm_count();
+  n.own_slots = (n.tc && D == 64 ? 4 : 3) * sm_count();
+  n.own_per_item = Kh * (n.tc ? (group + 7) / 8 : 1);
+  const int tiles = int(int64_t(B) * group / n.tile_rows) + B / 2 + 1;
+  n.prefix_items = 2 * n.prefix_slots / Kh + tiles;
+  n.own_items = 4 * n.own_slots / n.own_per_item + B;
+  // a prefix CTA leaves at most tile_rows rows of parts
+  n.prefix_parts = 2 * int64_t(B) + 2 * int64_t(n.prefix_slots) * n.tile_rows / H;
   n.own_parts = n.own_items;
   return n;
 }
 
+// Least cost C such that pieces of at most C fit in `fit` CTAs, at most `waves` waves of
+// them: tries one wave after the other, each with a fixed cost, and keeps the cheapest.
+// count(C) falls as C grows.
+template <typename F>
+int64_t best_piece(int64_t least, int64_t most, int64_t slots, int max_waves, int64_t overhead,
+                   F count) {
+  int64_t best = -1, best_cost = 0;
+  for (int waves = 1; waves <= max_waves; ++waves) {
+    if (count(most) > slots * waves) continue;
+    int64_t lo = least, hi = most;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      if (count(mid) <= slots * waves)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    const int64_t cost = waves * (lo + overhead);
+    if (best < 0 || cost < best_cost) {
+      best = lo;
+      best_cost = cost;
+    }
+  }
+  return best < 0 ? most : best;
+}
+
 int64_t plan_ints(const Limits& n, int B) {
-  return kHeader + int64_t(B) * (kRowInts + 1) + int64_t(n.prefix_items) * kPrefixInts +
-         int64_t(n.own_items) * kOwnInts;
+  return kHeader + (int64_t(B) + 3) / 4 * 4 +
+         (int64_t(n.prefix_items) + n.own_items) * kItemInts;
 }
 
 bool sizes_ok(int B, int H, int Kh, int D, int dtype) {
@@ -388,7 +421,9 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
   // C++ allocations below may throw; nothing may leave a C entry that way
   try {
     struct Group {
-      int first, size, blocks, tiles, splits, chunk;
+      int first, size, blocks, tiles, tile_rows, splits, chunk;
+      int64_t cost;  // of a 128-key tile, in softmax passes over 128 rows
+      bool halves;   // one tile of at most 128 rows: two halves of the keys side by side
     };
     std::vector<Group> groups;
     std::vector<int> shared(B, 0), seen(B, 0);
@@ -412,8 +447,14 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
       }
       // one member, or nothing shared: its keys are its own
       if (hi - lo < 2 || prefix_blocks[i] == 0) continue;
-      Group g{int(list.size()), hi - lo, prefix_blocks[i], 0, 0, 0};
-      g.tiles = int((int64_t(g.size) * group + n.tile_rows - 1) / n.tile_rows);
+      Group g{int(list.size()), hi - lo, prefix_blocks[i], 0, 0, 0, 0, 1, false};
+      const int rows = g.size * group;
+      g.tiles = (rows + n.tile_rows - 1) / n.tile_rows;
+      g.tile_rows = (rows + g.tiles - 1) / g.tiles;  // even tiles
+      if (n.tc) {
+        g.halves = rows <= n.tile_rows / 2;
+        g.cost = g.halves ? 1 : 2;
+      }
       for (int j = lo; j < hi; ++j) {
         list.push_back(members[j]);
         shared[members[j]] = g.blocks;
@@ -423,81 +464,94 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
     for (int b = 0; b < B; ++b)
       if (row_blocks[b] < 0) return fail(AS_ERR_INVALID_ARG, "%s: negative row_blocks", who);
 
-    // prefix splits: about prefix_slots CTAs in all, and within the workspace's parts
-    int64_t work = 0;
-    for (const Group& g : groups) work += int64_t(g.tiles) * g.blocks * Kh;
-    int64_t chunk = std::max<int64_t>(n.min_prefix, (work + n.prefix_slots - 1) / n.prefix_slots);
-    for (;; chunk += chunk / 2) {
-      int64_t parts = 0;
+    // prefix splits: pieces of about equal cost, in units of 8 blocks
+    auto split_prefix = [&](int64_t piece) -> int64_t {
+      int64_t ctas = 0;
       for (Group& g : groups) {
-        g.splits = int(std::min<int64_t>(kMaxSplits, (g.blocks + chunk - 1) / chunk));
-        g.chunk = (g.blocks + g.splits - 1) / g.splits;
+        const int units = (g.blocks + 7) / 8;
+        const int most = kMaxSplits / (g.halves ? 2 : 1);
+        const int splits = int(std::min<int64_t>(most, (units * g.cost + piece - 1) / piece));
+        g.chunk = (units + splits - 1) / splits * 8;
         g.splits = (g.blocks + g.chunk - 1) / g.chunk;
-        parts += int64_t(g.splits) * g.size;
+        ctas += int64_t(g.splits) * g.tiles * Kh;
       }
-      if (parts <= n.prefix_parts) break;
+      return ctas;
+    };
+    if (!groups.empty()) {
+      int64_t most = 2;
+      for (const Group& g : groups) most = std::max(most, (g.blocks + 7) / 8 * g.cost);
+      int64_t piece = best_piece(2, most, n.prefix_slots, 2, kPrefixOverhead, split_prefix);
+      for (;; piece += (piece + 1) / 2) {  // and within the workspace's parts and the items
+        const int64_t ctas = split_prefix(piece);
+        int64_t parts = 0;
+        for (const Group& g : groups) parts += int64_t(g.splits) * g.size * (g.halves ? 2 : 1);
+        if (parts <= n.prefix_parts && ctas / Kh <= n.prefix_items) break;
+      }
     }
-    int64_t own_work = 0;
-    for (int b = 0; b < B; ++b) own_work += int64_t(row_blocks[b] - shared[b]) * Kh;
-    const int64_t own_chunk =
-        std::max<int64_t>(n.min_own, (own_work + n.own_slots - 1) / n.own_slots);
+    auto own_splits = [&](int b, int64_t piece) -> int {
+      const int64_t blocks = row_blocks[b] - shared[b];
+      return int(std::clamp<int64_t>((blocks + piece - 1) / piece, 1, kMaxSplits));
+    };
+    int64_t own_most = kMinOwn;
+    for (int b = 0; b < B; ++b) own_most = std::max<int64_t>(own_most, row_blocks[b] - shared[b]);
+    const int64_t own_piece =
+        best_piece(kMinOwn, own_most, n.own_slots, 4, kOwnOverhead, [&](int64_t piece) {
+          int64_t items = 0;
+          for (int b = 0; b < B; ++b) items += own_splits(b, piece);
+          return items * n.own_per_item;
+        });
 
     std::fill(plan, plan + kHeader, 0);
-    int32_t* rows = plan + kHeader;
-    std::fill(rows, rows + int64_t(B) * kRowInts, 0);
-    int32_t* mem = rows + int64_t(B) * kRowInts;
-    std::fill(mem, mem + B, 0);
+    int32_t* mem = plan + kHeader;
+    const int mem_ints = (B + 3) / 4 * 4;
+    auto* pre = reinterpret_cast<PrefixItem*>(mem + mem_ints);
+    auto* own = reinterpret_cast<OwnItem*>(pre + n.prefix_items);
+    std::fill(mem, mem + (plan_ints(n, B) - kHeader), 0);
     std::copy(list.begin(), list.end(), mem);
-    int32_t* pre = mem + B;
-    int32_t* own = pre + int64_t(n.prefix_items) * kPrefixInts;
+    std::vector<OwnItem> row_items(B, OwnItem{});
     int n_pre = 0, n_own = 0, most = 0;
-    int64_t part = 0;
+    int part = 0;
     for (const Group& g : groups) {
+      const int ways = g.halves ? 2 : 1;
       most = std::max(most, g.blocks);
       for (int i = 0; i < g.size; ++i) {
-        int32_t* r = rows + int64_t(list[g.first + i]) * kRowInts;
-        r[kRShared] = g.blocks;
-        r[kRPrefixSplits] = g.splits;
-        r[kRPrefixPart] = int32_t(part + i);
-        r[kRPrefixStep] = g.size;
+        OwnItem& r = row_items[list[g.first + i]];
+        r.shared = g.blocks;
+        r.prefix_splits = g.splits * ways;
+        r.prefix_part = part + i;
+        r.prefix_step = g.size;
       }
       const int all_rows = g.size * group;
       for (int s = 0; s < g.splits; ++s)
         for (int t = 0; t < g.tiles; ++t) {
-          int32_t* it = pre + int64_t(n_pre++) * kPrefixInts;
-          std::fill(it, it + kPrefixInts, 0);
-          it[kPMembers] = g.first;
-          it[kPRow0] = t * n.tile_rows;
-          it[kPRows] = std::min(n.tile_rows, all_rows - t * n.tile_rows);
-          it[kPBegin] = s * g.chunk;
-          it[kPEnd] = std::min(g.blocks, (s + 1) * g.chunk);
-          it[kPPart] = int32_t(part + int64_t(s) * g.size);
+          PrefixItem& it = pre[n_pre++];
+          it.table_row = list[g.first];
+          it.members = g.first;
+          it.row0 = t * g.tile_rows;
+          it.rows = std::min(g.tile_rows, all_rows - t * g.tile_rows);
+          it.begin = s * g.chunk;
+          it.end = std::min(g.blocks, (s + 1) * g.chunk);
+          it.part = part + s * ways * g.size;
+          it.step = g.halves ? g.size : 0;
         }
-      part += int64_t(g.splits) * g.size;
+      part += g.splits * ways * g.size;
     }
     // own items, the longest first so that the last to start are short
-    struct Own {
-      int row, split, blocks;
-    };
-    std::vector<Own> items;
-    int64_t own_part = 0;
+    std::vector<std::pair<int64_t, OwnItem>> items;
+    int own_part = 0;
     for (int b = 0; b < B; ++b) {
-      const int blocks = row_blocks[b] - shared[b];
-      const int splits = std::clamp<int>(int((blocks + own_chunk - 1) / own_chunk), 1, kMaxSplits);
-      int32_t* r = rows + int64_t(b) * kRowInts;
-      r[kROwnSplits] = splits;
-      r[kROwnPart] = int32_t(own_part);
-      if (splits > 1) own_part += splits;
-      for (int s = 0; s < splits; ++s) items.push_back({b, s, (blocks + splits - 1) / splits});
+      const int64_t blocks = row_blocks[b] - shared[b];
+      OwnItem& r = row_items[b];
+      r.row = b;
+      r.own_splits = own_splits(b, own_piece);
+      r.own_part = own_part;
+      if (r.own_splits > 1) own_part += r.own_splits;
+      for (r.split = 0; r.split < r.own_splits; ++r.split)
+        items.push_back({(blocks + r.own_splits - 1) / r.own_splits, r});
     }
     std::stable_sort(items.begin(), items.end(),
-                     [](const Own& x, const Own& y) { return x.blocks > y.blocks; });
-    for (const Own& x : items) {
-      int32_t* it = own + int64_t(n_own++) * kOwnInts;
-      std::fill(it, it + kOwnInts, 0);
-      it[kORow] = x.row;
-      it[kOSplit] = x.split;
-    }
+                     [](const auto& x, const auto& y) { return x.first > y.first; });
+    for (const auto& x : items) own[n_own++] = x.second;
     plan[kHMagic] = kMagic;
     plan[kHSeqs] = B;
     plan[kHHeads] = H;
@@ -508,14 +562,13 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
     plan[kHOwnItems] = n_own;
     plan[kHPrefixGrid] = full_grid ? n.prefix_items : n_pre;
     plan[kHOwnGrid] = full_grid ? n.own_items : n_own;
-    plan[kHOffRows] = kHeader;
     plan[kHOffMembers] = int32_t(mem - plan);
-    plan[kHOffPrefix] = int32_t(pre - plan);
-    plan[kHOffOwn] = int32_t(own - plan);
+    plan[kHOffPrefix] = int32_t(reinterpret_cast<int32_t*>(pre) - plan);
+    plan[kHOffOwn] = int32_t(reinterpret_cast<int32_t*>(own) - plan);
     plan[kHPrefixParts] = int32_t(n.prefix_parts);
     plan[kHOwnParts] = int32_t(n.own_parts);
     plan[kHTileRows] = n.tile_rows;
-    plan[kHInts] = int32_t((own - plan) + int64_t(n.own_items) * kOwnInts);
+    plan[kHInts] = int32_t(plan_ints(n, B));
     plan[kHMostShared] = most;
   } catch (...) {
     return fail(AS_ERR_INVALID_ARG, "%s: out of host memory", who);
@@ -549,6 +602,8 @@ extern "C" int as_shared_prefix_decode_attention(
   if (h[kHMagic] != kMagic || h[kHSeqs] != num_seqs || h[kHHeads] != num_heads ||
       h[kHKvHeads] != num_kv_heads || h[kHDim] != head_dim || h[kHDtype] != dtype)
     return fail(AS_ERR_INVALID_ARG, "%s: the plan was made for another batch", who);
+  if (reinterpret_cast<uintptr_t>(plan) & 15)
+    return fail(AS_ERR_INVALID_ARG, "%s: the plan must be 16-byte aligned", who);
   if (h[kHMostShared] > max_blocks)
     return fail(AS_ERR_INVALID_ARG, "%s: the plan shares %d blocks, the table holds %d", who,
                 h[kHMostShared], max_blocks);
@@ -563,7 +618,9 @@ extern "C" int as_shared_prefix_decode_attention(
     return fail(AS_ERR_INVALID_ARG, "%s: workspace must be 256-byte aligned", who);
 
   Args a{};
-  a.plan = plan;
+  a.members = plan + h[kHOffMembers];
+  a.prefix_items = reinterpret_cast<const PrefixItem*>(plan + h[kHOffPrefix]);
+  a.own_items = reinterpret_cast<const OwnItem*>(plan + h[kHOffOwn]);
   a.bt = block_tables;
   a.bt_stride = bt_stride;
   a.seq_lens = seq_lens_k;

@@ -16,27 +16,33 @@ namespace sp {
 constexpr int kBS = 16;  // tokens per block
 constexpr int kMagic = 0x53504c31;
 
-// Plan: kHeader ints, then per batch row kRowInts, the members of all groups, the
-// prefix items (kPrefixInts each) and the own items (kOwnInts each).
+// Plan: kHeader ints, then the members of all groups, the prefix items and the own
+// items.  An item holds all that its block needs to start, so a block reaches its first
+// K / V load after one plan read; an unused item is all zero.
 constexpr int kHeader = 32;
 enum Header {
   kHMagic, kHSeqs, kHHeads, kHKvHeads, kHDim, kHDtype, kHPrefixItems, kHOwnItems, kHPrefixGrid,
-  kHOwnGrid, kHOffRows, kHOffMembers, kHOffPrefix, kHOffOwn, kHPrefixParts, kHOwnParts,
-  kHTileRows, kHInts, kHMostShared
+  kHOwnGrid, kHOffMembers, kHOffPrefix, kHOffOwn, kHPrefixParts, kHOwnParts, kHTileRows, kHInts,
+  kHMostShared
 };
-constexpr int kRowInts = 8;
-enum RowInfo {
-  kRShared,       // shared blocks at the front of the row's table
-  kRPrefixSplits, // parts those were split into
-  kRPrefixPart,   // part index of the first of them (a part holds H heads)
-  kRPrefixStep,   // part indexes from one split to the next
-  kROwnSplits,
-  kROwnPart
+constexpr int kItemInts = 8;
+struct PrefixItem {
+  int table_row;  // batch row whose table names the blocks (the group's first member)
+  int members;    // its group's first entry in the members
+  int row0, rows; // query rows (member, head of the KV head) of the group
+  int begin, end; // blocks
+  int part;       // part index of the group's first member (a part holds H heads)
+  int step;       // > 0: two halves of the keys go to parts `step` apart
 };
-constexpr int kPrefixInts = 8;
-enum PrefixItem { kPMembers, kPRow0, kPRows, kPBegin, kPEnd, kPPart };
-constexpr int kOwnInts = 4;
-enum OwnItem { kORow, kOSplit };
+struct OwnItem {
+  int row, split;     // batch row, and which of its own_splits ranges
+  int shared;         // shared blocks at the front of its table
+  int prefix_splits;  // parts those were divided into,
+  int prefix_part;    // the first one's index
+  int prefix_step;    // and the distance to the next
+  int own_splits;     // 0: unused item
+  int own_part;
+};
 
 // Parts in the workspace: counters, then (m, l) and o of every (part, head); the prefix
 // parts come first.
@@ -47,7 +53,9 @@ struct Parts {
 };
 
 struct Args {
-  const int32_t* plan;
+  const PrefixItem* prefix_items;
+  const OwnItem* own_items;
+  const int32_t* members;
   const int32_t* bt;
   int64_t bt_stride;
   const int32_t* seq_lens;
@@ -63,29 +71,42 @@ struct Args {
   uint64_t wait_limit;
 };
 
+template <typename Item>
+__device__ __forceinline__ Item load_item(const Item* items, int i) {
+  static_assert(sizeof(Item) == 4 * kItemInts, "item size");
+  alignas(16) Item it;
+  const int4* src = reinterpret_cast<const int4*>(items + i);
+  reinterpret_cast<int4*>(&it)[0] = __ldg(src);
+  reinterpret_cast<int4*>(&it)[1] = __ldg(src + 1);
+  return it;
+}
+
 // A row's own keys and what of its shared part counts.  A row shorter than its group's
 // shared part takes nothing from it: all its keys are its own.
 struct RowPlan {
   int shared, prefix_splits, prefix_part, prefix_step, own_splits, own_part;
-  int len, blocks;
+  int len, begin, count;  // keys; this item's blocks
 };
-__device__ __forceinline__ RowPlan row_plan(const Args& a, int b, bool flag) {
-  const int32_t* r = a.plan + a.plan[kHOffRows] + b * kRowInts;
+__device__ __forceinline__ RowPlan row_plan(const Args& a, const OwnItem& it, bool flag) {
   RowPlan p;
-  p.shared = r[kRShared];
-  p.prefix_splits = r[kRPrefixSplits];
-  p.prefix_part = r[kRPrefixPart];
-  p.prefix_step = r[kRPrefixStep];
-  p.own_splits = r[kROwnSplits];
-  p.own_part = a.own_part0 + r[kROwnPart];
-  p.len = max(0, a.seq_lens[b]);
-  p.blocks = (p.len + kBS - 1) / kBS;
-  if (p.blocks > a.max_blocks) {
+  p.shared = it.shared;
+  p.prefix_splits = it.prefix_splits;
+  p.prefix_part = it.prefix_part;
+  p.prefix_step = it.prefix_step;
+  p.own_splits = it.own_splits;
+  p.own_part = a.own_part0 + it.own_part;
+  p.len = max(0, a.seq_lens[it.row]);
+  int blocks = (p.len + kBS - 1) / kBS;
+  if (blocks > a.max_blocks) {
     if (flag) flag_status(a.status, kStatusBadLength);
-    p.blocks = a.max_blocks;
+    blocks = a.max_blocks;
     p.len = a.max_blocks * kBS;
   }
   if (p.len < p.shared * kBS) p.shared = p.prefix_splits = 0;
+  const int own = blocks - p.shared;
+  const int per = (own + p.own_splits - 1) / p.own_splits;
+  p.begin = p.shared + min(own, it.split * per);
+  p.count = p.shared + min(own, (it.split + 1) * per) - p.begin;
   return p;
 }
 
@@ -232,7 +253,7 @@ __device__ void finish_own(const Args& a, const RowPlan& p, T* __restrict__ out,
 }
 
 // Tensor-core launches (shared_prefix_tc.cu): 16-bit types, head_dim 64 or 128.
-constexpr int kTcTileRows = 128;
+constexpr int kTcTileRows = 256;
 inline bool tc_geometry(int D, int dtype) {
   return (dtype == AS_DTYPE_BF16 || dtype == AS_DTYPE_F16) && (D == 64 || D == 128);
 }

@@ -1,12 +1,14 @@
 // (9) Shared-prefix decode attention on tensor cores: bf16 / fp16, head_dim 64 or 128.
 //
 // Prefix launch (sp_prefix_kernel).  A group's members' query heads of KV head g are the
-// rows of a matrix: a tile of 128 of them attends over one range of the shared blocks
-// with tcgen05.mma, S = Q K^T into TMEM, softmax by four warps (one row per thread),
-// P back into TMEM as the A operand of O += P V.  K / V tiles arrive by TMA, block by
-// block.  Roles: warp 0 loads, warp 1 issues MMAs, warps 2-5 softmax.  Two blocks share
-// an SM (about 100 KB of shared memory and 256 TMEM columns each), so one's
-// exponentials overlap the other's products and waits.
+// rows of a matrix that attends over the shared blocks.  A block runs two softmax
+// streams of 128 rows: the two halves of a tile of up to 256 rows, which share every
+// K / V tile, or, for a group of at most 128 rows, the same rows twice over the even
+// and the odd key tiles.  S = Q K^T by tcgen05.mma into TMEM, P back into TMEM as the A
+// operand of O += P V; K / V arrive by TMA, paged block by paged block.  Roles (320
+// threads, one block per SM): warp 0 loads K / V, warp 1 issues MMAs by polling which
+// stream is ready, warps 2-5 and 6-9 the streams' softmax, one row per thread, the two
+// warps of an SM sub-partition taking turns on its exponent unit.
 //
 // Own launch (sp_own_kernel).  One sequence, up to 8 query heads of a KV head: too few
 // rows for tcgen05, and bound by reading K / V once; the decode kernel's warp-level
@@ -38,29 +40,33 @@ constexpr float kLazySlack = 8.0f;  // log2 units a row's scores may exceed its 
 template <int HD>
 struct PreCfg {
   static constexpr int D = HD;
-  static constexpr int kBN = D == 64 ? 128 : 64;  // keys per tile: 32 KB of K and V
+  static constexpr int kBN = 128;                 // keys per tile
   static constexpr int kBlocks = kBN / kBS;
   static constexpr int kSub = D / 64;             // 128-byte-wide swizzle sub-tiles
   static constexpr int kQSub = 128 * 128;
   static constexpr int kKVSub = kBN * 128;
-  static constexpr int kQBytes = kSub * kQSub;
+  static constexpr int kQBytes = kSub * kQSub;    // 128 rows
   static constexpr int kKVBytes = kSub * kKVSub;  // K (or V) of one tile
-  static constexpr int kStages = 2;
-  static constexpr int kOffKV = kQBytes;
+  static constexpr int kStages = D == 64 ? 4 : 2;  // even: a stage always serves one stream
+  static constexpr int kOffKV = 2 * kQBytes;
   static constexpr int kOffBar = kOffKV + kStages * 2 * kKVBytes;
   static constexpr int kSmemBytes = kOffBar + 256;
-  static constexpr int kThreads = 192;
-  // TMEM columns: S [0, kBN), P (16-bit pairs) after it, O the last D of 256
-  static constexpr int kCols = 256;
-  static constexpr int kColP = kBN;
-  static constexpr int kColO = kCols - D;
-  static_assert(kBN + kBN / 2 + D <= kCols, "TMEM columns");
-  static_assert(2 * (kSmemBytes + 1024) <= 227 * 1024, "two blocks per SM");
+  static constexpr int kThreads = 320;
+  // TMEM columns of a stream, from 256 i: S [0, 128), P (16-bit pairs), O the last D.  At
+  // D = 128 they do not fit side by side: P overwrites S, already in registers, and
+  // S(j+1) is issued after PV(j), which reads P, in the MMA thread's order.
+  static constexpr int kCols = 512;
+  static constexpr bool kAliasP = kBN + kBN / 2 > 256 - D;
+  static constexpr int kColP = kAliasP ? 0 : kBN;
+  static constexpr int kColO = 256 - D;
+  static_assert(kSmemBytes + 1024 <= 227 * 1024, "shared memory");
 };
 
 struct PreBars {
-  uint64_t kv_full[2], kv_empty[2];
-  uint64_t s_full, s_free, p_full, pv_done, drain;
+  uint64_t kv_full[4], kv_empty[4];
+  uint64_t s_full[2], s_free[2], p_full[2], pv_done[2];
+  uint64_t turn[2][4];  // hand-off of the exponent unit between a sub-partition's warps
+  uint64_t drain;
   uint32_t tmem;
   int abort;
 };
@@ -69,7 +75,7 @@ static_assert(sizeof(PreBars) <= 256, "barrier block");
 __device__ __forceinline__ bool stopped(volatile int* flag) { return *flag != 0; }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(192, 2)
+__global__ void __launch_bounds__(320, 1)
 sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
                  const __grid_constant__ CUtensorMap tmap_v, const T* __restrict__ q,
                  const Args a, float scale_log2, int starve) {
@@ -78,33 +84,41 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kIdescS = tc::idesc_f16(kBF16, 128, BN, false, false);
   constexpr uint32_t kIdescO = tc::idesc_f16(kBF16, 128, D, false, true);
-  pdl_wait();
-  pdl_trigger();  // every block of this launch has started: the own launch may start
-
-  const int32_t* plan = a.plan;
-  if (int(blockIdx.x) >= plan[kHPrefixItems]) return;
-  const int32_t* it = plan + plan[kHOffPrefix] + blockIdx.x * kPrefixInts;
-  const int32_t* members = plan + plan[kHOffMembers] + it[kPMembers];
-  const int row0 = it[kPRow0], rows = it[kPRows];
-  const int begin = it[kPBegin], end = it[kPEnd], part = it[kPPart];
-  const int g = blockIdx.y, group = a.group;
-  const int n_tiles = (end - begin + NB - 1) / NB;
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   PreBars* bars = reinterpret_cast<PreBars*>(smem + Cfg::kOffBar);
   volatile int* abort_flag = &bars->abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int active = (rows + 31) / 32;  // softmax warps with rows
+
+  pdl_wait();
+  pdl_trigger();  // every block of this launch has started: the own launch may start
+  const PrefixItem it = load_item(a.prefix_items, blockIdx.x);
+  if (it.rows == 0) return;
+  const int g = blockIdx.y, group = a.group;
+  const int n_tiles = (it.end - it.begin + NB - 1) / NB;
+  const bool halves = it.step > 0;
+  // streams: rows and key tiles of each; stream i's tile j is key tile stride * j + i * odd
+  const int rows0 = min(it.rows, 128);
+  const int rows1 = halves ? rows0 : it.rows - rows0;
+  const int stride = halves ? 2 : 1, odd = halves ? 1 : 0;
+  const int n0 = halves ? (n_tiles + 1) / 2 : n_tiles;
+  const int n1 = halves ? n_tiles / 2 : (rows1 > 0 ? n_tiles : 0);
+  const int active0 = (rows0 + 31) / 32, active1 = (rows1 + 31) / 32;  // warps with rows
+
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&bars->kv_full[s], 1);
       mbar_init(&bars->kv_empty[s], 1);
     }
-    mbar_init(&bars->s_full, 1);
-    mbar_init(&bars->s_free, active);
-    mbar_init(&bars->p_full, active);
-    mbar_init(&bars->pv_done, 1);
+    for (int i = 0; i < 2; ++i) {
+      const int n = max(1, i ? active1 : active0);
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->s_free[i], n);
+      mbar_init(&bars->p_full[i], n);
+      mbar_init(&bars->pv_done[i], 1);
+      for (int w = 0; w < 4; ++w) mbar_init(&bars->turn[i][w], 1);
+    }
     mbar_init(&bars->drain, 1);
     bars->abort = 0;
     fence_mbarrier_init();
@@ -113,15 +127,69 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
     tc::tmem_alloc(&bars->tmem, Cfg::kCols);
     tc::tmem_relinquish();
   }
-  // Q rows (member, head) into the 128B-swizzled layout; rows past the tile are zero
-  {
+
+  int issued = 0;
+  auto load_tiles = [&](int j0, int j1) {  // warp 0: key tiles [j0, j1)
+    const int32_t* row = a.bt + int64_t(it.table_row) * a.bt_stride;
+    // blocks past the range: any block of it (finite as the rest), masked below
+    const int first = __ldg(row + it.begin);
+    const int fill = first >= 0 && first < a.num_blocks ? first : 0;
+    auto load_id = [&](int j) -> int {
+      const int blk = it.begin + NB * j + (lane & (NB - 1));
+      int id = fill;
+      if (blk < it.end) {
+        id = __ldg(row + blk);
+        if (id < 0 || id >= a.num_blocks) {
+          flag_status(a.status, kStatusBadBlockId);
+          id = fill;
+        }
+      }
+      return id;
+    };
+    const uint64_t policy = l2_policy_evict_last();  // other row tiles read them too
+    int id = load_id(j0);
+    for (int j = j0; j < j1; ++j) {
+      const int st = j % NS;
+      const bool ready =
+          j < NS || (!stopped(abort_flag) &&
+                     mbar_wait(&bars->kv_empty[st], ((j / NS) + 1) & 1, a.status, a.wait_limit));
+      if (!__all_sync(0xffffffffu, ready)) {
+        *abort_flag = 1;
+        break;
+      }
+      if (lane == 0) mbar_arrive_expect_tx(&bars->kv_full[st], 2 * Cfg::kKVBytes);
+      __syncwarp();
+      uint8_t* stage = smem + Cfg::kOffKV + st * 2 * Cfg::kKVBytes;
+      if (lane < NB) {
+#pragma unroll
+        for (int sb = 0; sb < Cfg::kSub; ++sb) {
+          tma_load_4d(stage + sb * Cfg::kKVSub + lane * 2048, &tmap_k, &bars->kv_full[st], sb * 64,
+                      g, 0, id, policy);
+          tma_load_4d(stage + Cfg::kKVBytes + sb * Cfg::kKVSub + lane * 2048, &tmap_v,
+                      &bars->kv_full[st], sb * 64, g, 0, id, policy);
+        }
+      }
+      issued = j + 1;
+      if (j + 1 < j1) id = load_id(j + 1);
+      __syncwarp();
+    }
+  };
+  const int ahead = min(NS, n_tiles);
+  if (warp == 0) {
+    // the first ring of K / V, while the other warps bring in Q
+    __syncwarp();  // the barriers were initialised by lane 0
+    if (!starve) load_tiles(0, ahead);
+  } else if (warp >= 2) {
+    // Q rows (member, head) into the 128B-swizzled layout; rows past a tile are zero
+    const int32_t* members = a.members + it.members;
     const bool vec = ((reinterpret_cast<uintptr_t>(q) | uintptr_t(a.q_stride * 2)) & 15) == 0;
-    for (int i = threadIdx.x; i < 128 * (D / 8); i += Cfg::kThreads) {
+    const int tile_rows = halves ? 128 : 256;
+    for (int i = threadIdx.x - 64; i < tile_rows * (D / 8); i += Cfg::kThreads - 64) {
       const int r = i / (D / 8), c = i - r * (D / 8);
       uint4 x = make_uint4(0, 0, 0, 0);
-      if (r < rows) {
-        const int rr = row0 + r;
-        const T* src = q + int64_t(members[rr / group]) * a.q_stride +
+      if (r < it.rows) {
+        const int rr = it.row0 + r;
+        const T* src = q + int64_t(__ldg(members + rr / group)) * a.q_stride +
                        int64_t(g * group + rr % group) * D + c * 8;
         if (vec) {
           x = *reinterpret_cast<const uint4*>(src);
@@ -131,8 +199,8 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
           for (int j = 0; j < 8; ++j) e[j] = src[j];
         }
       }
-      *reinterpret_cast<uint4*>(smem + (c >> 3) * Cfg::kQSub + r * 128 +
-                                (((c & 7) ^ (r & 7)) << 4)) = x;
+      *reinterpret_cast<uint4*>(smem + (r >> 7) * Cfg::kQBytes + (c >> 3) * Cfg::kQSub +
+                                (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
     }
     fence_proxy_async_smem();
   }
@@ -142,220 +210,218 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
   const uint32_t tmem = bars->tmem;
   const uint32_t sQ = smem_u32(smem), sKV = smem_u32(smem + Cfg::kOffKV);
 
-  int issued = 0;
   if (warp == 0) {
-    // ---------------------------------------------------------------- loads
-    if (!starve) {
-      if (lane == 0) {
-        tma_prefetch_desc(&tmap_k);
-        tma_prefetch_desc(&tmap_v);
-      }
-      const int32_t* row = a.bt + int64_t(members[0]) * a.bt_stride;
-      // blocks past the range: any block of it (finite as the rest), masked below
-      const int first = row[begin];
-      const int fill = first >= 0 && first < a.num_blocks ? first : 0;
-      auto load_id = [&](int j) -> int {
-        const int blk = begin + NB * j + (lane & (NB - 1));
-        int id = fill;
-        if (blk < end) {
-          id = __ldg(row + blk);
-          if (id < 0 || id >= a.num_blocks) {
-            flag_status(a.status, kStatusBadBlockId);
-            id = fill;
-          }
-        }
-        return id;
-      };
-      const uint64_t policy = l2_policy_evict_last();  // other row tiles read them too
-      int id = load_id(0);
-      for (int j = 0; j < n_tiles; ++j) {
-        const int st = j % NS;
-        const bool ready =
-            !stopped(abort_flag) &&
-            (j < NS || mbar_wait(&bars->kv_empty[st], ((j / NS) + 1) & 1, a.status, a.wait_limit));
-        if (!__all_sync(0xffffffffu, ready)) {
-          *abort_flag = 1;
-          break;
-        }
-        if (lane == 0) mbar_arrive_expect_tx(&bars->kv_full[st], 2 * Cfg::kKVBytes);
-        __syncwarp();
-        uint8_t* stage = smem + Cfg::kOffKV + st * 2 * Cfg::kKVBytes;
-        if (lane < NB) {
-#pragma unroll
-          for (int sb = 0; sb < Cfg::kSub; ++sb) {
-            tma_load_4d(stage + sb * Cfg::kKVSub + lane * 2048, &tmap_k, &bars->kv_full[st],
-                        sb * 64, g, 0, id, policy);
-            tma_load_4d(stage + Cfg::kKVBytes + sb * Cfg::kKVSub + lane * 2048, &tmap_v,
-                        &bars->kv_full[st], sb * 64, g, 0, id, policy);
-          }
-        }
-        issued = j + 1;
-        if (j + 1 < n_tiles) id = load_id(j + 1);
-        __syncwarp();
-      }
-    }
+    if (!starve && n_tiles > ahead) load_tiles(ahead, n_tiles);
   } else if (warp == 1) {
     // ----------------------------------------------------------------- MMAs
     if (lane == 0) {
-      auto issue_s = [&](int st) {
+      auto issue_s = [&](int i, int st) {
+        const uint32_t qi = sQ + (halves ? 0 : i) * Cfg::kQBytes;
         const uint32_t k = sKV + st * 2 * Cfg::kKVBytes;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          tc::mma_f16(tmem,
-                      tc::sdesc_sw128(sQ + (kk >> 2) * Cfg::kQSub + (kk & 3) * 32, 16, 1024),
+          tc::mma_f16(tmem + 256 * i,
+                      tc::sdesc_sw128(qi + (kk >> 2) * Cfg::kQSub + (kk & 3) * 32, 16, 1024),
                       tc::sdesc_sw128(k + (kk >> 2) * Cfg::kKVSub + (kk & 3) * 32, 16, 1024),
                       kIdescS, kk > 0 ? 1u : 0u);
       };
-      auto wait = [&](uint64_t* bar, int parity) -> bool {
-        return !stopped(abort_flag) && mbar_wait(bar, parity & 1, a.status, a.wait_limit);
-      };
-      bool ok = wait(&bars->kv_full[0], 0);
-      if (ok) {
-        issue_s(0);
-        tc::commit(&bars->s_full);
-      }
-      for (int j = 0; ok && j < n_tiles; ++j) {
-        if (j + 1 < n_tiles) {  // S of the next tile while the softmax works on this one
-          ok = wait(&bars->kv_full[(j + 1) % NS], (j + 1) / NS) && wait(&bars->s_free, j);
-          if (!ok) break;
-          tc::fence_after_sync();
-          issue_s((j + 1) % NS);
-          tc::commit(&bars->s_full);
-        }
-        ok = wait(&bars->p_full, j);
-        if (!ok) break;
-        tc::fence_after_sync();
-        const uint32_t v = sKV + (j % NS) * 2 * Cfg::kKVBytes + Cfg::kKVBytes;
+      auto issue_pv = [&](int i, int st, bool acc) {
+        const uint32_t v = sKV + st * 2 * Cfg::kKVBytes + Cfg::kKVBytes;
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
-          tc::mma_f16_ts(tmem + Cfg::kColO, tmem + Cfg::kColP + kk * 8,
+          tc::mma_f16_ts(tmem + 256 * i + Cfg::kColO, tmem + 256 * i + Cfg::kColP + kk * 8,
                          tc::sdesc_sw128(v + kk * 2048, Cfg::kKVSub, 1024), kIdescO,
-                         (j > 0 || kk > 0) ? 1u : 0u);
-        tc::commit(&bars->pv_done);
-        tc::commit(&bars->kv_empty[j % NS]);
+                         (acc || kk > 0) ? 1u : 0u);
+      };
+      const int nk[2] = {n0, n1};
+      int js[2] = {0, 0}, jp[2] = {0, 0};  // next S and next PV of each stream
+      bool ok = true;
+      uint64_t t_idle = 0;
+      uint32_t spin = 0;
+      while (jp[0] < nk[0] || jp[1] < nk[1]) {
+        if (stopped(abort_flag)) break;
+        bool did = false;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int j = js[i];
+          const int t = stride * j + odd * i;
+          if (j < nk[i] && (!Cfg::kAliasP || jp[i] >= j) &&
+              mbar_try_wait(&bars->kv_full[t % NS], (t / NS) & 1) &&
+              (j == 0 || mbar_try_wait(&bars->s_free[i], (j - 1) & 1))) {
+            tc::fence_after_sync();
+            issue_s(i, t % NS);
+            tc::commit(&bars->s_full[i]);
+            js[i] = j + 1;
+            did = true;
+          }
+          const int jq = jp[i];
+          if (jq < js[i] && mbar_try_wait(&bars->p_full[i], jq & 1)) {
+            const int tq = stride * jq + odd * i;
+            tc::fence_after_sync();
+            issue_pv(i, tq % NS, jq > 0);
+            tc::commit(&bars->pv_done[i]);
+            jp[i] = jq + 1;
+            did = true;
+            // a stage is free once every stream that reads it has issued its PV
+            if (halves || jp[1 - i] > jq || jq >= nk[1 - i]) tc::commit(&bars->kv_empty[tq % NS]);
+          }
+        }
+        if (did) {
+          spin = 0;
+        } else if ((++spin & 255u) == 0u) {  // the timer is slow to read: rarely
+          const uint64_t now = global_timer_ns();
+          if (spin == 256u) {
+            t_idle = now;
+          } else if (now - t_idle > a.wait_limit) {
+            flag_status(a.status, kStatusWaitTimeout);
+            ok = false;
+            break;
+          }
+        }
       }
       if (!ok) *abort_flag = 1;
       tc::commit(&bars->drain);
       mbar_wait(&bars->drain, 0, a.status, a.wait_limit);
     }
     __syncwarp();
-  } else if ((warp & 3) < active) {
+  } else {
     // -------------------------------------------------------------- softmax
-    const int quad = warp & 3;  // the TMEM lanes this warp may access
+    const int i = (warp - 2) >> 2;  // stream
+    const int quad = warp & 3;      // the TMEM lanes this warp may access
     const int r = quad * 32 + lane;
-    const uint32_t tS = tmem + (uint32_t(quad * 32) << 16);
-    const uint32_t tP = tS + Cfg::kColP, tO = tS + Cfg::kColO;
-    float m = -INFINITY, l = 0.f;
-    bool ok = true;
-    for (int j = 0; j < n_tiles; ++j) {
-      const bool go = !stopped(abort_flag) &&
-                      mbar_wait(&bars->s_full, j & 1, a.status, a.wait_limit);
-      if (!__all_sync(0xffffffffu, go)) {
-        ok = false;
-        break;
-      }
-      tc::fence_after_sync();
-      float x[BN];
-      {
-        uint32_t v[BN / 32][32];
-#pragma unroll
-        for (int u = 0; u < BN / 32; ++u) tc::ld_32x32b_x32(tS + 32 * u, v[u]);
-        tc::wait_ld();
-#pragma unroll
-        for (int u = 0; u < BN / 32; ++u)
-#pragma unroll
-          for (int c = 0; c < 32; ++c) x[32 * u + c] = __uint_as_float(v[u][c]);
-      }
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->s_free);
-      const int keys = (end - begin) * kBS - j * BN;  // of this tile
-      if (keys < BN) {
-#pragma unroll
-        for (int c = 0; c < BN; ++c) x[c] = c < keys ? x[c] : -INFINITY;
-      }
-      float mp[8];
-#pragma unroll
-      for (int c = 0; c < 8; ++c) mp[c] = fmaxf(x[c], x[8 + c]);
-#pragma unroll
-      for (int c = 16; c < BN; c += 16)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) mp[e] = max3f(mp[e], x[c + e], x[c + 8 + e]);
-      const float mx = fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])),
-                             fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7])));
-      // lazy maximum: exponents stay below 2^8, within every type's range, unless a
-      // score exceeds the current one by more; then O and l are rescaled
-      float alpha = 1.f;
-      if (mx * scale_log2 > m + kLazySlack) {
-        const float m_new = mx * scale_log2;
-        alpha = fast_exp2(m - m_new);
-        m = m_new;
-      }
-      const float neg_m = m == -INFINITY ? 0.f : -m;
-      const uint64_t sc2 = f2_pack(scale_log2, scale_log2);
-      const uint64_t nm2 = f2_pack(neg_m, neg_m);
-      uint64_t sum2[4] = {0, 0, 0, 0};
-      uint32_t pk[BN / 2];
-#pragma unroll
-      for (int c = 0; c < BN / 2; ++c) {
-        float e0, e1;
-        f2_unpack(f2_fma(f2_pack(x[2 * c], x[2 * c + 1]), sc2, nm2), e0, e1);
-        const float p0 = fast_exp2(e0), p1 = fast_exp2(e1);
-        sum2[c & 3] = f2_add(sum2[c & 3], f2_pack(p0, p1));
-        pk[c] = pack2<T>(p0, p1);
-      }
-      float s0, s1;
-      f2_unpack(f2_add(f2_add(sum2[0], sum2[1]), f2_add(sum2[2], sum2[3])), s0, s1);
-      if (j > 0) {  // the product with V of the last tile still reads P and writes O
-        if (!__all_sync(0xffffffffu,
-                        mbar_wait(&bars->pv_done, (j - 1) & 1, a.status, a.wait_limit))) {
+    const int my_rows = i ? rows1 : rows0, n = i ? n1 : n0;
+    if (quad < (i ? active1 : active0)) {
+      const uint32_t tS = tmem + 256 * i + (uint32_t(quad * 32) << 16);
+      const uint32_t tP = tS + Cfg::kColP, tO = tS + Cfg::kColO;
+      const bool partner = quad < (i ? active0 : active1);
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int j = 0; j < n; ++j) {
+        const bool go = !stopped(abort_flag) &&
+                        mbar_wait(&bars->s_full[i], j & 1, a.status, a.wait_limit);
+        if (!__all_sync(0xffffffffu, go)) {
           ok = false;
           break;
         }
         tc::fence_after_sync();
-      }
+        float x[BN];
+        {
+          uint32_t v[BN / 32][32];
 #pragma unroll
-      for (int u = 0; u < BN / 64; ++u)
-        tc::st_32x32b_x32(tP + 32 * u, *reinterpret_cast<const uint32_t(*)[32]>(&pk[32 * u]));
-      l = l * alpha + (s0 + s1);
-      if (j > 0 && __any_sync(0xffffffffu, alpha < 1.f)) {
+          for (int u = 0; u < BN / 32; ++u) tc::ld_32x32b_x32(tS + 32 * u, v[u]);
+          tc::wait_ld();
+#pragma unroll
+          for (int u = 0; u < BN / 32; ++u)
+#pragma unroll
+            for (int c = 0; c < 32; ++c) x[32 * u + c] = __uint_as_float(v[u][c]);
+        }
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->s_free[i]);
+        const int keys = (it.end - it.begin) * kBS - (stride * j + odd * i) * BN;  // of this tile
+        if (keys < BN) {
+#pragma unroll
+          for (int c = 0; c < BN; ++c) x[c] = c < keys ? x[c] : -INFINITY;
+        }
+        float mp[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) mp[c] = fmaxf(x[c], x[8 + c]);
+#pragma unroll
+        for (int c = 16; c < BN; c += 16)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mp[e] = max3f(mp[e], x[c + e], x[c + 8 + e]);
+        const float mx = fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])),
+                               fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7])));
+        // lazy maximum: exponentials stay below 2^8, within every type's range, unless a
+        // score exceeds the current one by more; then O and l are rescaled
+        float alpha = 1.f;
+        if (mx * scale_log2 > m + kLazySlack) {
+          const float m_new = mx * scale_log2;
+          alpha = fast_exp2(m - m_new);
+          m = m_new;
+        }
+        const float neg_m = m == -INFINITY ? 0.f : -m;
+        // a warp waits only for a hand-off that its partner will make
+        if (partner && (i == 0 ? (j >= 1 && j - 1 < n1) : j < n0)) {
+          const bool mine = !stopped(abort_flag) &&
+                            mbar_wait(&bars->turn[i][quad], (i == 0 ? j - 1 : j) & 1, a.status,
+                                      a.wait_limit);
+          if (!__all_sync(0xffffffffu, mine)) {
+            ok = false;
+            break;
+          }
+        }
+        const uint64_t sc2 = f2_pack(scale_log2, scale_log2);
+        const uint64_t nm2 = f2_pack(neg_m, neg_m);
+        uint64_t sum2[4] = {0, 0, 0, 0};
+        uint32_t pk[BN / 2];
+#pragma unroll
+        for (int c = 0; c < BN / 2; ++c) {
+          float e0, e1;
+          f2_unpack(f2_fma(f2_pack(x[2 * c], x[2 * c + 1]), sc2, nm2), e0, e1);
+          const float p0 = fast_exp2(e0), p1 = fast_exp2(e1);
+          sum2[c & 3] = f2_add(sum2[c & 3], f2_pack(p0, p1));
+          pk[c] = pack2<T>(p0, p1);
+          if (c == BN / 4 - 1) {  // half-way: the partner's start overlaps the rest
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->turn[1 - i][quad]);
+          }
+        }
+        float s0, s1;
+        f2_unpack(f2_add(f2_add(sum2[0], sum2[1]), f2_add(sum2[2], sum2[3])), s0, s1);
+        if (j > 0) {  // the product with V of the last tile still reads P and writes O
+          if (!__all_sync(0xffffffffu,
+                          mbar_wait(&bars->pv_done[i], (j - 1) & 1, a.status, a.wait_limit))) {
+            ok = false;
+            break;
+          }
+          tc::fence_after_sync();
+        }
+#pragma unroll
+        for (int u = 0; u < BN / 64; ++u)
+          tc::st_32x32b_x32(tP + 32 * u, *reinterpret_cast<const uint32_t(*)[32]>(&pk[32 * u]));
+        l = l * alpha + (s0 + s1);
+        if (j > 0 && __any_sync(0xffffffffu, alpha < 1.f)) {
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tc::ld_32x32b_x32(tO + c * 32, o);
+            tc::wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tc::st_32x32b_x32(tO + c * 32, o);
+          }
+        }
+        tc::wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->p_full[i]);
+      }
+      if (!ok) *abort_flag = 1;
+      const bool done =
+          ok && n > 0 && __all_sync(0xffffffffu, mbar_wait(&bars->pv_done[i], (n - 1) & 1,
+                                                           a.status, a.wait_limit));
+      if (ok && n > 0 && !done) *abort_flag = 1;
+      const int rr = it.row0 + (halves ? 0 : 128 * i) + r;
+      const int part = it.part + i * it.step + rr / group;
+      const size_t at = size_t(part) * a.H + g * group + rr % group;
+      if (done) {
+        tc::fence_after_sync();
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           tc::ld_32x32b_x32(tO + c * 32, o);
           tc::wait_ld();
+          if (r < my_rows) {
+            uint4* dst = reinterpret_cast<uint4*>(a.parts.o + at * D + c * 32);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-          tc::st_32x32b_x32(tO + c * 32, o);
+            for (int e = 0; e < 8; ++e)
+              dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
         }
       }
-      tc::wait_st();
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->p_full);
+      if (r < my_rows) a.parts.ml[at] = done ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
     }
-    if (!ok) *abort_flag = 1;
-    const bool done = ok && __all_sync(0xffffffffu, mbar_wait(&bars->pv_done, (n_tiles - 1) & 1,
-                                                              a.status, a.wait_limit));
-    if (ok && !done) *abort_flag = 1;
-    const int rr = row0 + r;
-    const size_t at = (size_t(part) + rr / group) * a.H + g * group + rr % group;
-    if (done) {
-      tc::fence_after_sync();
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        tc::ld_32x32b_x32(tO + c * 32, o);
-        tc::wait_ld();
-        if (r < rows) {
-          uint4* dst = reinterpret_cast<uint4*>(a.parts.o + at * D + c * 32);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-        }
-      }
-    }
-    if (r < rows) a.parts.ml[at] = done ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
     tc::fence_before_sync();
   }
 
@@ -364,7 +430,7 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem, Cfg::kCols);
   }
-  if (warp == 0 && lane == 0 && *abort_flag) {  // let the copies in flight land
+  if (warp == 0 && lane == 0 && stopped(abort_flag)) {  // let the copies in flight land
     for (int j = max(0, issued - NS); j < issued; ++j)
       mbar_wait(&bars->kv_full[j % NS], (j / NS) & 1, a.status, a.wait_limit);
   }
@@ -403,22 +469,18 @@ sp_own_kernel(const __grid_constant__ CUtensorMap tmap_k,
   }
   // Without the wait: everything read below was written before the prefix launch, whose
   // blocks let this launch start only after their own wait for it.
-  const int32_t* plan = a.plan;
-  if (int(blockIdx.x) >= plan[kHOwnItems]) {
+  const OwnItem it = load_item(a.own_items, blockIdx.x);
+  if (it.own_splits == 0) {
     pdl_wait();
     return;
   }
-  const int32_t* it = plan + plan[kHOffOwn] + blockIdx.x * kOwnInts;
-  const int b = it[kORow], split = it[kOSplit];
+  const int b = it.row, split = it.split;
   const int chunks = (a.group + Cfg::kHeads - 1) / Cfg::kHeads;
   const int g = blockIdx.y / chunks, chunk = blockIdx.y - g * chunks;
   const int h0 = g * a.group + chunk * Cfg::kHeads;
   const int heads = min(Cfg::kHeads, a.group - chunk * Cfg::kHeads);
-  const RowPlan rp = row_plan(a, b, threadIdx.x == 0 && split == 0 && blockIdx.y == 0);
-  const int own = rp.blocks - rp.shared;
-  const int per = (own + rp.own_splits - 1) / rp.own_splits;
-  const int begin = rp.shared + min(own, split * per);
-  const int count = rp.shared + min(own, (split + 1) * per) - begin;
+  const RowPlan rp = row_plan(a, it, threadIdx.x == 0 && split == 0 && blockIdx.y == 0);
+  const int begin = rp.begin, count = rp.count;
   const int n_iter = (count + W - 1) / W;
 
   extern __shared__ uint8_t smem_raw[];

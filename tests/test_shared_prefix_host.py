@@ -11,7 +11,7 @@ from agentserve_b200 import _native as N
 from agentserve_b200 import ops
 
 HEADER = 32
-ROW, PREFIX, OWN = 8, 8, 4
+ITEM = 8
 
 
 @pytest.fixture(scope="module")
@@ -27,52 +27,59 @@ def plan_of(groups, prefix, rows, H=32, Kh=8, D=64, dtype=torch.bfloat16, **kw):
 
 
 def check_covers(p, groups, prefix, rows):
-    """Every (member, head of a KV head, shared block) is in one prefix item, its part
-    indexes are disjoint and in range, and every row has all its own items."""
+    """Every (member, head of a KV head, shared block) is in one prefix item, the parts
+    that items write are disjoint, in range and those the row's own items join, and every
+    row has all its own items."""
     h = p._host.tolist()
     B, H, Kh = h[1:4]
     group = H // Kh
-    n_pre, n_own, off_rows, off_mem, off_pre, off_own = h[6], h[7], h[10], h[11], h[12], h[13]
-    assert h[17] <= p._host.numel()
-    info = [h[off_rows + ROW * b: off_rows + ROW * (b + 1)] for b in range(B)]
+    n_pre, n_own, off_mem, off_pre, off_own = h[6], h[7], h[10], h[11], h[12]
+    most_prefix, most_own, tile = h[13], h[14], h[15]
+    assert h[16] <= p._host.numel() and off_pre % 4 == 0 and off_own % 4 == 0
     want = {}
     for m, n in zip(groups, prefix):
         if len(m) >= 2 and n > 0:
             for b in m:
-                want[b] = n
+                want[b] = (n, set(m))
+    own, used = {}, set()
+    for i in range(n_own):
+        it = h[off_own + ITEM * i: off_own + ITEM * (i + 1)]
+        assert it[6] > 0
+        own.setdefault(it[0], []).append(it)
+    for b in range(B):
+        items = sorted(own[b], key=lambda x: x[1])
+        assert [x[1] for x in items] == list(range(items[0][6]))
+        assert all(x[2:] == items[0][2:] for x in items)
+        if b not in want:
+            assert items[0][2:4] == [0, 0]
+        if items[0][6] > 1:
+            mine = set(range(items[0][7], items[0][7] + items[0][6]))
+            assert not mine & used and max(mine) < most_own
+            used |= mine
+    assert not any(h[off_own + ITEM * n_own: h[16]])  # unused items are zero
     seen, parts = {}, {}
     for i in range(n_pre):
-        first, row0, n_rows, begin, end, part = h[off_pre + PREFIX * i: off_pre + PREFIX * i + 6]
-        assert 0 < n_rows <= h[16] and 0 <= begin < end
+        row, first, row0, n_rows, begin, end, part, step = h[off_pre + ITEM * i:
+                                                             off_pre + ITEM * (i + 1)]
+        assert 0 < n_rows <= tile and 0 <= begin < end
         for r in range(row0, row0 + n_rows):
             b = h[off_mem + first + r // group]
-            index = part + r // group
-            assert 0 <= index < h[14]
-            assert (index - info[b][2]) % info[b][3] == 0
-            assert 0 <= (index - info[b][2]) // info[b][3] < info[b][1]
-            assert parts.setdefault((index, r % group), (b, begin, end)) == (b, begin, end)
-            seen.setdefault((b, r % group), []).append((begin, end))
+            assert row in want[b][1]
+            _, _, shared, splits, part0, apart, _, _ = own[b][0]
+            assert shared == want[b][0]
+            for index in [part + r // group] + ([part + step + r // group] if step else []):
+                assert 0 <= index < most_prefix
+                assert (index - part0) % apart == 0 and 0 <= (index - part0) // apart < splits
+                assert parts.setdefault((index, r % group), i) == i
+            seen.setdefault((b, r % group), []).append((begin, end, 2 if step else 1))
+    assert not any(h[off_pre + ITEM * n_pre: off_own])
     assert set(b for b, _ in seen) == set(want)
-    for b, n in want.items():
-        assert info[b][0] == n
+    for b, (n, _) in want.items():
         for e in range(group):
             spans = sorted(seen[b, e])
-            assert len(spans) == info[b][1]
+            assert sum(x[2] for x in spans) == own[b][0][3] <= 64
             assert spans[0][0] == 0 and spans[-1][1] == n
             assert all(x[1] == y[0] for x, y in zip(spans, spans[1:]))
-    splits = {}
-    used = set()
-    for i in range(n_own):
-        b, s = h[off_own + OWN * i: off_own + OWN * i + 2]
-        splits.setdefault(b, []).append(s)
-    for b in range(B):
-        assert sorted(splits[b]) == list(range(info[b][4]))
-        if b not in want:
-            assert info[b][:2] == [0, 0]
-        if info[b][4] > 1:
-            mine = set(range(info[b][5], info[b][5] + info[b][4]))
-            assert not mine & used and max(mine) < h[15]
-            used |= mine
     return h
 
 

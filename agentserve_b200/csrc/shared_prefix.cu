@@ -53,6 +53,7 @@ __global__ void __launch_bounds__(kThreads)
 sp_generic_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restrict__ k_cache,
                   const T* __restrict__ v_cache, const Args a) {
   using Cfg = GenCfg<DP, RW, TG>;
+  static_assert(!kPrefix || TG == 1, "a prefix item leaves one result");
   constexpr int EPL = DP / 32;
   if (kPrefix || a.wait_first) {
     pdl_wait();
@@ -205,7 +206,7 @@ sp_generic_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], off);
 
-  // token groups joined in shared memory
+  // the token groups' results in shared memory, for the join
   __syncthreads();
   float* ro = smem;                                  // [TG][rows][DP]
   float* rm = ro + TG * Cfg::kRows * DP;             // [TG][rows]
@@ -221,32 +222,6 @@ sp_generic_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
     }
   }
   __syncthreads();
-  if (TG > 1) {
-    for (int r = warp; r < Cfg::kRows; r += kNWarps) {
-      float M = -INFINITY, L = 0.f;
-      for (int t = 0; t < TG; ++t) M = fmaxf(M, rm[t * Cfg::kRows + r]);
-      float acc[EPL];
-#pragma unroll
-      for (int e = 0; e < EPL; ++e) acc[e] = 0.f;
-      if (M != -INFINITY) {
-        for (int t = 0; t < TG; ++t) {
-          const int at = t * Cfg::kRows + r;
-          const float w = expf(rm[at] - M);
-          L += w * rl[at];
-#pragma unroll
-          for (int e = 0; e < EPL; ++e) acc[e] += w * ro[at * DP + lane + 32 * e];
-        }
-      }
-      __syncwarp();
-#pragma unroll
-      for (int e = 0; e < EPL; ++e) ro[r * DP + lane + 32 * e] = acc[e];
-      if (lane == 0) {
-        rm[r] = M;
-        rl[r] = L;
-      }
-    }
-    __syncthreads();
-  }
   if (kPrefix) {
     for (int i = threadIdx.x; i < rows * D; i += kThreads) {
       const int r = i / D, d = i - r * D, rr = row0 + r;
@@ -260,7 +235,7 @@ sp_generic_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
     }
     return;
   }
-  finish_own<T, false, Cfg::kRows, kThreads>(a, rp, out, b, split, g * group + row0, rows, ro, DP,
+  finish_own<T, false, Cfg::kRows, kThreads, TG>(a, rp, out, b, split, g * group + row0, rows, ro, DP,
                                              rm, rl, smem + Cfg::kJoin);
   pdl_wait();  // this launch ends after the prefix launch before it
 }
@@ -332,7 +307,8 @@ Limits limits(int B, int H, int Kh, int D, int dtype) {
   n.prefix_slots = (n.tc ? 1 : 2) * sm_count();
   n.own_slots = (n.tc && D == 64 ? 4 : 3) * sm_count();
   n.own_per_item = Kh * (n.tc ? (group + 7) / 8 : 1);
-  const int tiles = int(int64_t(B) * group / n.tile_rows) + B / 2 + 1;
+  const int per_tile = std::max(1, n.tile_rows / group) * group;  // rows, whole members
+  const int tiles = int(int64_t(B) * group / std::min(per_tile, n.tile_rows)) + B + 1;
   n.prefix_items = 2 * n.prefix_slots / Kh + tiles;
   n.own_items = 4 * n.own_slots / n.own_per_item + B;
   // a prefix CTA leaves at most tile_rows rows of parts
@@ -447,19 +423,27 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
       }
       // one member, or nothing shared: its keys are its own
       if (hi - lo < 2 || prefix_blocks[i] == 0) continue;
-      Group g{int(list.size()), hi - lo, prefix_blocks[i], 0, 0, 0, 0, 1, false};
-      const int rows = g.size * group;
-      g.tiles = (rows + n.tile_rows - 1) / n.tile_rows;
-      g.tile_rows = (rows + g.tiles - 1) / g.tiles;  // even tiles
-      if (n.tc) {
-        g.halves = rows <= n.tile_rows / 2;
-        g.cost = g.halves ? 1 : 2;
+      // Whole members to a tile.  On tensor cores a pass over 256 rows costs twice one
+      // over 128, so a rest of at most 128 rows is a group of its own, at half the cost.
+      const int per_tile = std::max(1, n.tile_rows / group);
+      const int full = (hi - lo) / per_tile * per_tile;
+      for (int first = lo; first < hi;) {
+        const int size = n.tc && first == lo && full > 0 ? full : hi - first;
+        Group g{int(list.size()), size, prefix_blocks[i], 0, 0, 0, 0, 1, false};
+        const int rows = size * group;
+        g.tile_rows = group > n.tile_rows ? n.tile_rows : per_tile * group;
+        g.tiles = (rows + g.tile_rows - 1) / g.tile_rows;
+        if (n.tc) {
+          g.halves = rows <= n.tile_rows / 2;
+          g.cost = g.halves ? 1 : 2;
+        }
+        for (int j = first; j < first + size; ++j) {
+          list.push_back(members[j]);
+          shared[members[j]] = g.blocks;
+        }
+        groups.push_back(g);
+        first += size;
       }
-      for (int j = lo; j < hi; ++j) {
-        list.push_back(members[j]);
-        shared[members[j]] = g.blocks;
-      }
-      groups.push_back(g);
     }
     for (int b = 0; b < B; ++b)
       if (row_blocks[b] < 0) return fail(AS_ERR_INVALID_ARG, "%s: negative row_blocks", who);
@@ -480,7 +464,8 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
     if (!groups.empty()) {
       int64_t most = 2;
       for (const Group& g : groups) most = std::max(most, (g.blocks + 7) / 8 * g.cost);
-      int64_t piece = best_piece(2, most, n.prefix_slots, 2, kPrefixOverhead, split_prefix);
+      int64_t piece = best_piece(n.tc ? 2 : 1, most, n.prefix_slots, 2, n.tc ? kPrefixOverhead : 1,
+                                 split_prefix);
       for (;; piece += (piece + 1) / 2) {  // and within the workspace's parts and the items
         const int64_t ctas = split_prefix(piece);
         int64_t parts = 0;
@@ -495,7 +480,8 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
     int64_t own_most = kMinOwn;
     for (int b = 0; b < B; ++b) own_most = std::max<int64_t>(own_most, row_blocks[b] - shared[b]);
     const int64_t own_piece =
-        best_piece(kMinOwn, own_most, n.own_slots, 4, kOwnOverhead, [&](int64_t piece) {
+        best_piece(n.tc ? kMinOwn : 2, own_most, n.own_slots, 4, n.tc ? kOwnOverhead : 4,
+                   [&](int64_t piece) {
           int64_t items = 0;
           for (int b = 0; b < B; ++b) items += own_splits(b, piece);
           return items * n.own_per_item;

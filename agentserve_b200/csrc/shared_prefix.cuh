@@ -123,28 +123,42 @@ constexpr int kMaxSplits = 64;
 // Shared-memory floats a join works in.
 constexpr int join_scratch(int rows, int threads) { return rows * 2 * kMaxSplits + 4 * threads; }
 
-// Ends an own item: rows [h0, h0 + nr) of sequence b, nr <= kRows, whose part of split
-// `split` is in shared memory (o [nr][ld], m, l).  Joins it with the other parts of the
-// rows when it is the last to arrive, and writes the output.  All threads of the block
-// call this.  A warp per row turns the parts' (m, l) into weights; then every thread
-// sums its share of the parts for four dimensions of a row, so the loads of the parts,
-// which come from L2, are all in flight at once.  scratch: join_scratch() floats of
-// shared memory, apart from o, m and l.
-template <typename T, bool kBase2, int kRows, int kThreads>
+// Ends an own item: rows [h0, h0 + nr) of sequence b.  Its part of split `split` is in
+// shared memory as kSub results over different keys (o [kSub][kRows][D], rows D apart
+// by ld, m and l [kSub][kRows]).  Joins them with the other parts of the rows, when it is
+// the last of the row's own items to arrive, and writes the output.  All threads of the
+// block call this.  A warp per row turns the (m, l) into weights; then every thread sums
+// its share of the parts for four dimensions of a row, eight loads in flight, as the
+// parts come from L2.  scratch: join_scratch() floats of shared memory, 16-byte aligned,
+// apart from o, m and l.
+template <typename T, bool kBase2, int kRows, int kThreads, int kSub>
 __device__ void finish_own(const Args& a, const RowPlan& p, T* __restrict__ out, int b, int split,
-                           int h0, int nr, const float* o, int ld, const float* m,
-                           const float* l, float* scratch) {
+                           int h0, int nr, const float* o, int ld, const float* m, const float* l,
+                           float* scratch) {
   __shared__ int s_last;
   auto s_w = reinterpret_cast<float(*)[2 * kMaxSplits]>(scratch + 4 * kThreads);
-  float4* s_sum = reinterpret_cast<float4*>(scratch);  // 16-byte aligned
+  float4* s_sum = reinterpret_cast<float4*>(scratch);
   const int D = a.D, H = a.H;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool alone = p.own_splits == 1;
   if (!alone) {
+    // this item's part: its results relative to their common maximum
     for (int i = threadIdx.x; i < nr * D; i += kThreads) {
       const int r = i / D, d = i - r * D;
+      float M = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll
+      for (int w = 0; w < kSub; ++w) M = fmaxf(M, m[w * kRows + r]);
+#pragma unroll
+      for (int w = 0; w < kSub; ++w) {
+        const float x = m[w * kRows + r];
+        if (x == -INFINITY) continue;
+        const float e = part_exp<kBase2>(x - M);
+        L += e * l[w * kRows + r];
+        O += e * o[(w * kRows + r) * ld + d];
+      }
       const size_t at = size_t(p.own_part + split) * H + h0 + r;
-      a.parts.o[at * D + d] = o[r * ld + d];
-      if (d == 0) a.parts.ml[at] = make_float2(m[r], l[r]);
+      a.parts.o[at * D + d] = O;
+      if (d == 0) a.parts.ml[at] = make_float2(M, L);
     }
     // the barrier orders this block's stores before thread 0's fence, which publishes
     // them before the arrival; the last arriver fences again before its reads
@@ -159,8 +173,9 @@ __device__ void finish_own(const Args& a, const RowPlan& p, T* __restrict__ out,
     if (threadIdx.x == 0) a.parts.counters[b * H + h0] = 0;  // for the next call
   }
   if (p.prefix_splits > 0 && !a.wait_first) pdl_wait();  // the prefix parts are written
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int np = p.prefix_splits + (alone ? 1 : p.own_splits);
+  // parts in global memory, then (alone) this item's results in shared memory
+  const int ng = p.prefix_splits + (alone ? 0 : p.own_splits);
+  const int np = ng + (alone ? kSub : 0);
   const auto part = [&](int s) -> size_t {
     return s < p.prefix_splits ? size_t(p.prefix_part) + size_t(s) * p.prefix_step
                                : size_t(p.own_part + s - p.prefix_splits);
@@ -172,9 +187,10 @@ __device__ void finish_own(const Args& a, const RowPlan& p, T* __restrict__ out,
     for (int i = 0; i < 2 * kMaxSplits / 32; ++i) {
       const int s = lane + 32 * i;
       ml[i] = make_float2(-INFINITY, 0.f);
-      if (s < np)
-        ml[i] = alone && s == np - 1 ? make_float2(m[r], l[r])
-                                     : __ldcg(&a.parts.ml[part(s) * H + h0 + r]);
+      if (s < ng)
+        ml[i] = __ldcg(&a.parts.ml[part(s) * H + h0 + r]);
+      else if (s < np)
+        ml[i] = make_float2(m[(s - ng) * kRows + r], l[(s - ng) * kRows + r]);
       M = fmaxf(M, ml[i].x);
     }
 #pragma unroll
@@ -187,54 +203,72 @@ __device__ void finish_own(const Args& a, const RowPlan& p, T* __restrict__ out,
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
-    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);  // NaN stays NaN
+    const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
     for (int i = 0; i < 2 * kMaxSplits / 32; ++i)
       if (lane + 32 * i < np) s_w[r][lane + 32 * i] = ml[i].x * inv;
   }
   __syncthreads();
   if ((D & 3) == 0) {
-    const int nv = nr * (D / 4);
+    const int dv = D >> 2, nv = nr * dv;
+    const bool packed =
+        a.os_d == 1 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0;
     for (int v0 = 0; v0 < nv; v0 += kThreads) {
       // as many threads as there are vectors share out the parts
       const int here = min(nv - v0, kThreads), ways = kThreads / here;
-      const int v = v0 + threadIdx.x % here, way = threadIdx.x / here;
-      const int r = v / (D / 4), d = (v - r * (D / 4)) * 4;
+      const int way = threadIdx.x / here;
+      const int v = v0 + threadIdx.x - way * here;
+      const int r = v / dv, d = (v - r * dv) * 4;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      const auto add = [&](float w, const float4& x) {
+        acc.x += w * x.x;
+        acc.y += w * x.y;
+        acc.z += w * x.z;
+        acc.w += w * x.w;
+      };
       if (way < ways) {
-#pragma unroll 4
-        for (int s = way; s < np; s += ways) {
+        const float* base = a.parts.o + size_t(h0 + r) * D + d;
+        for (int s0 = way; s0 < ng; s0 += 8 * ways) {
+          float4 x[8];
+          float w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int s = s0 + e * ways;
+            w[e] = s < ng ? s_w[r][s] : 0.f;
+            x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (w[e] != 0.f)  // a part without keys holds no values
+              x[e] = __ldcg(reinterpret_cast<const float4*>(base + part(s) * H * D));
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) add(w[e], x[e]);
+        }
+        for (int s = ng + way; s < np; s += ways) {
           const float w = s_w[r][s];
-          if (w == 0.f) continue;  // a part without keys holds no values
-          const float4 x =
-              alone && s == np - 1
-                  ? make_float4(o[r * ld + d], o[r * ld + d + 1], o[r * ld + d + 2],
-                                o[r * ld + d + 3])
-                  : __ldcg(reinterpret_cast<const float4*>(
-                        &a.parts.o[(part(s) * H + h0 + r) * D + d]));
-          acc.x += w * x.x;
-          acc.y += w * x.y;
-          acc.z += w * x.z;
-          acc.w += w * x.w;
+          if (w == 0.f) continue;
+          add(w, *reinterpret_cast<const float4*>(o + ((s - ng) * kRows + r) * ld + d));
         }
       }
-      s_sum[threadIdx.x] = acc;
-      __syncthreads();
-      if (threadIdx.x < here) {
-        for (int y = 1; y < ways; ++y) {
-          const float4 x = s_sum[threadIdx.x + y * here];
-          acc.x += x.x;
-          acc.y += x.y;
-          acc.z += x.z;
-          acc.w += x.w;
-        }
+      if (ways > 1) {
+        s_sum[threadIdx.x] = acc;
+        __syncthreads();
+        if (way == 0)
+          for (int y = 1; y < ways; ++y) add(1.f, s_sum[threadIdx.x + y * here]);
+      }
+      if (way == 0) {
         T* dst = out + size_t(b) * H * D + size_t(h0 + r) * a.os_h + size_t(d) * a.os_d;
-        dst[0] = Elem<T>::from_f32(acc.x);
-        dst[a.os_d] = Elem<T>::from_f32(acc.y);
-        dst[2 * size_t(a.os_d)] = Elem<T>::from_f32(acc.z);
-        dst[3 * size_t(a.os_d)] = Elem<T>::from_f32(acc.w);
+        T val[4] = {Elem<T>::from_f32(acc.x), Elem<T>::from_f32(acc.y), Elem<T>::from_f32(acc.z),
+                    Elem<T>::from_f32(acc.w)};
+        if (packed) {
+          struct alignas(4 * sizeof(T)) Four {
+            T v[4];
+          };
+          *reinterpret_cast<Four*>(dst) = Four{val[0], val[1], val[2], val[3]};
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dst[size_t(e) * a.os_d] = val[e];
+        }
       }
-      __syncthreads();
+      if (v0 + kThreads < nv) __syncthreads();
     }
     return;
   }
@@ -244,8 +278,8 @@ __device__ void finish_own(const Args& a, const RowPlan& p, T* __restrict__ out,
     for (int s = 0; s < np; ++s) {
       const float w = s_w[r][s];
       if (w == 0.f) continue;
-      acc += w * (alone && s == np - 1 ? o[r * ld + d]
-                                       : __ldcg(&a.parts.o[(part(s) * H + h0 + r) * D + d]));
+      acc += w * (s < ng ? __ldcg(&a.parts.o[(part(s) * H + h0 + r) * D + d])
+                         : o[((s - ng) * kRows + r) * ld + d]);
     }
     out[size_t(b) * H * D + size_t(h0 + r) * a.os_h + size_t(d) * a.os_d] =
         Elem<T>::from_f32(acc);

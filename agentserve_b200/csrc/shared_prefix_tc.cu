@@ -123,96 +123,103 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
     bars->abort = 0;
     fence_mbarrier_init();
   }
-  if (warp == 1) {
-    tc::tmem_alloc(&bars->tmem, Cfg::kCols);
-    tc::tmem_relinquish();
-  }
+  __syncthreads();  // the barriers are initialised
 
   int issued = 0;
-  auto load_tiles = [&](int j0, int j1) {  // warp 0: key tiles [j0, j1)
-    const int32_t* row = a.bt + int64_t(it.table_row) * a.bt_stride;
-    // blocks past the range: any block of it (finite as the rest), masked below
-    const int first = __ldg(row + it.begin);
-    const int fill = first >= 0 && first < a.num_blocks ? first : 0;
-    auto load_id = [&](int j) -> int {
-      const int blk = it.begin + NB * j + (lane & (NB - 1));
-      int id = fill;
-      if (blk < it.end) {
-        id = __ldg(row + blk);
-        if (id < 0 || id >= a.num_blocks) {
-          flag_status(a.status, kStatusBadBlockId);
-          id = fill;
-        }
-      }
-      return id;
-    };
-    const uint64_t policy = l2_policy_evict_last();  // other row tiles read them too
-    int id = load_id(j0);
-    for (int j = j0; j < j1; ++j) {
-      const int st = j % NS;
-      const bool ready =
-          j < NS || (!stopped(abort_flag) &&
-                     mbar_wait(&bars->kv_empty[st], ((j / NS) + 1) & 1, a.status, a.wait_limit));
-      if (!__all_sync(0xffffffffu, ready)) {
-        *abort_flag = 1;
-        break;
-      }
-      if (lane == 0) mbar_arrive_expect_tx(&bars->kv_full[st], 2 * Cfg::kKVBytes);
-      __syncwarp();
-      uint8_t* stage = smem + Cfg::kOffKV + st * 2 * Cfg::kKVBytes;
-      if (lane < NB) {
-#pragma unroll
-        for (int sb = 0; sb < Cfg::kSub; ++sb) {
-          tma_load_4d(stage + sb * Cfg::kKVSub + lane * 2048, &tmap_k, &bars->kv_full[st], sb * 64,
-                      g, 0, id, policy);
-          tma_load_4d(stage + Cfg::kKVBytes + sb * Cfg::kKVSub + lane * 2048, &tmap_v,
-                      &bars->kv_full[st], sb * 64, g, 0, id, policy);
-        }
-      }
-      issued = j + 1;
-      if (j + 1 < j1) id = load_id(j + 1);
-      __syncwarp();
-    }
-  };
-  const int ahead = min(NS, n_tiles);
   if (warp == 0) {
-    // the first ring of K / V, while the other warps bring in Q
-    __syncwarp();  // the barriers were initialised by lane 0
-    if (!starve) load_tiles(0, ahead);
-  } else if (warp >= 2) {
-    // Q rows (member, head) into the 128B-swizzled layout; rows past a tile are zero
-    const int32_t* members = a.members + it.members;
-    const bool vec = ((reinterpret_cast<uintptr_t>(q) | uintptr_t(a.q_stride * 2)) & 15) == 0;
-    const int tile_rows = halves ? 128 : 256;
-    for (int i = threadIdx.x - 64; i < tile_rows * (D / 8); i += Cfg::kThreads - 64) {
-      const int r = i / (D / 8), c = i - r * (D / 8);
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (r < it.rows) {
-        const int rr = it.row0 + r;
-        const T* src = q + int64_t(__ldg(members + rr / group)) * a.q_stride +
-                       int64_t(g * group + rr % group) * D + c * 8;
-        if (vec) {
-          x = *reinterpret_cast<const uint4*>(src);
-        } else {
-          T* e = reinterpret_cast<T*>(&x);
+    // ------------------------------------------------- K / V loads, from now on
+    if (!starve) {
+      if (lane == 0) {
+        tma_prefetch_desc(&tmap_k);
+        tma_prefetch_desc(&tmap_v);
+      }
+      const int32_t* row = a.bt + int64_t(it.table_row) * a.bt_stride;
+      // 32 block ids at a time, one per lane, read ahead of their use.  Blocks past the
+      // range: its last one (finite as the rest), masked below; an id outside the pool is
+      // flagged and block 0 read in its place.
+      const auto load_ids = [&](int j) -> int {
+        const int id = __ldg(row + min(it.begin + NB * j + lane, it.end - 1));
+        if (id >= 0 && id < a.num_blocks) return id;
+        flag_status(a.status, kStatusBadBlockId);
+        return 0;
+      };
+      constexpr int kPer = 32 / NB;  // tiles per read
+      const uint64_t policy = l2_policy_evict_last();  // other row tiles read them too
+      int ids = load_ids(0), next = n_tiles > kPer ? load_ids(kPer) : 0;
+      for (int j = 0; j < n_tiles; ++j) {
+        const int st = j % NS;
+        const bool ready =
+            !stopped(abort_flag) &&
+            (j < NS || mbar_wait(&bars->kv_empty[st], ((j / NS) + 1) & 1, a.status, a.wait_limit));
+        if (!__all_sync(0xffffffffu, ready)) {
+          *abort_flag = 1;
+          break;
+        }
+        if (j > 0 && j % kPer == 0) {
+          ids = next;
+          if (j + kPer < n_tiles) next = load_ids(j + kPer);
+        }
+        const int id = __shfl_sync(0xffffffffu, ids, (j % kPer) * NB + (lane & (NB - 1)));
+        if (lane == 0) mbar_arrive_expect_tx(&bars->kv_full[st], 2 * Cfg::kKVBytes);
+        __syncwarp();
+        uint8_t* stage = smem + Cfg::kOffKV + st * 2 * Cfg::kKVBytes;
+        if (lane < NB) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) e[j] = src[j];
+          for (int sb = 0; sb < Cfg::kSub; ++sb) {
+            tma_load_4d(stage + sb * Cfg::kKVSub + lane * 2048, &tmap_k, &bars->kv_full[st],
+                        sb * 64, g, 0, id, policy);
+            tma_load_4d(stage + Cfg::kKVBytes + sb * Cfg::kKVSub + lane * 2048, &tmap_v,
+                        &bars->kv_full[st], sb * 64, g, 0, id, policy);
+          }
+        }
+        issued = j + 1;
+        __syncwarp();
+      }
+    }
+  } else if (warp == 1) {
+    tc::tmem_alloc(&bars->tmem, Cfg::kCols);
+    tc::tmem_relinquish();
+  } else if (warp >= 2) {
+    // Q rows (member, head) into the 128B-swizzled layout, a thread per row or half row,
+    // all copies in flight at once; rows past a tile are zero
+    const int t = threadIdx.x - 64;
+    const int r = halves ? t & 127 : t;
+    const int c0 = halves && t >= 128 ? D / 16 : 0, c1 = halves && t < 128 ? D / 16 : D / 8;
+    uint8_t* dst = smem + (r >> 7) * Cfg::kQBytes + (r & 127) * 128;
+    const auto chunk = [&](int c) -> uint8_t* {
+      return dst + (c >> 3) * Cfg::kQSub + (((c & 7) ^ (r & 7)) << 4);
+    };
+    if (r < it.rows) {
+      const int rr = it.row0 + r;
+      const T* src = q + int64_t(__ldg(a.members + it.members + rr / group)) * a.q_stride +
+                     int64_t(g * group + rr % group) * D;
+      if (((reinterpret_cast<uintptr_t>(q) | uintptr_t(a.q_stride * 2)) & 15) == 0) {
+#pragma unroll 4
+        for (int c = c0; c < c1; ++c) cp_async_16(smem_u32(chunk(c)), src + c * 8);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+      } else {
+        for (int c = c0; c < c1; ++c) {
+          T e[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) e[j] = src[c * 8 + j];
+          memcpy(chunk(c), e, 16);
         }
       }
-      *reinterpret_cast<uint4*>(smem + (r >> 7) * Cfg::kQBytes + (c >> 3) * Cfg::kQSub +
-                                (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+    } else {
+      for (int c = c0; c < c1; ++c) *reinterpret_cast<uint4*>(chunk(c)) = make_uint4(0, 0, 0, 0);
     }
     fence_proxy_async_smem();
   }
-  tc::fence_before_sync();
-  __syncthreads();
-  tc::fence_after_sync();
-  const uint32_t tmem = bars->tmem;
+  uint32_t tmem = 0;
+  if (warp > 0) {  // Q and the TMEM address are there; the loads go on beside this
+    tc::fence_before_sync();
+    asm volatile("bar.sync 1, %0;" ::"n"(Cfg::kThreads - 32) : "memory");
+    tc::fence_after_sync();
+    tmem = bars->tmem;
+  }
   const uint32_t sQ = smem_u32(smem), sKV = smem_u32(smem + Cfg::kOffKV);
 
-  if (warp == 0) {
-    if (!starve && n_tiles > ahead) load_tiles(ahead, n_tiles);
-  } else if (warp == 1) {
+  if (warp == 1) {
     // ----------------------------------------------------------------- MMAs
     if (lane == 0) {
       auto issue_s = [&](int i, int st) {
@@ -284,7 +291,7 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
       mbar_wait(&bars->drain, 0, a.status, a.wait_limit);
     }
     __syncwarp();
-  } else {
+  } else if (warp > 1) {
     // -------------------------------------------------------------- softmax
     const int i = (warp - 2) >> 2;  // stream
     const int quad = warp & 3;      // the TMEM lanes this warp may access
@@ -604,7 +611,7 @@ sp_own_kernel(const __grid_constant__ CUtensorMap tmap_k,
   }
   __syncthreads();
 
-  // the warps' results joined in the stages' space: every copy has landed
+  // the warps' results in the stages' space: every copy has landed
   float* ro = reinterpret_cast<float*>(smem);        // [W][8][D]
   float* rm = ro + W * Cfg::kHeads * D;              // [W][8]
   float* rl = rm + W * Cfg::kHeads;
@@ -627,37 +634,8 @@ sp_own_kernel(const __grid_constant__ CUtensorMap tmap_k,
     }
   }
   __syncthreads();
-  float M[W], lw[W];  // this thread's row of the join
-  for (int idx = threadIdx.x; idx < heads * D; idx += Cfg::kThreads) {
-    const int h = idx / D, d = idx - h * D;
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < W; ++w) top = fmaxf(top, M[w] = rm[w * Cfg::kHeads + h]);
-    float acc = 0.f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      lw[w] = M[w] == -INFINITY ? 0.f : fast_exp2(M[w] - top);
-      if (lw[w] > 0.f) acc += lw[w] * ro[(w * Cfg::kHeads + h) * D + d];
-    }
-    ro[h * D + d] = acc;  // warp 0's value of this very element: read above by this thread
-  }
-  __syncthreads();
-  if (threadIdx.x < heads) {
-    const int h = threadIdx.x;
-    float top = -INFINITY, L = 0.f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) top = fmaxf(top, rm[w * Cfg::kHeads + h]);
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float x = rm[w * Cfg::kHeads + h];
-      if (x != -INFINITY) L += fast_exp2(x - top) * rl[w * Cfg::kHeads + h];
-    }
-    rm[h] = top;
-    rl[h] = L;
-  }
-  __syncthreads();
-  finish_own<T, true, Cfg::kHeads, Cfg::kThreads>(a, rp, out, b, split, h0, heads, ro, D, rm, rl,
-                                                  ro + Cfg::kJoinFloats);
+  finish_own<T, true, Cfg::kHeads, Cfg::kThreads, W>(a, rp, out, b, split, h0, heads, ro, D, rm,
+                                                     rl, ro + Cfg::kJoinFloats);
   pdl_wait();  // this launch ends after the prefix launch before it
 }
 

@@ -9,342 +9,697 @@
 // w >= min_p.  The row's token is the first kept one, in index order, at which the
 // running sum of kept weights exceeds u times their total.
 //
-// No sort: every filter keeps a prefix of one order, so a threshold on (x, number of
-// ties at x) describes it, and the threshold is found by histograms over a monotone
-// integer distance from the maximum, refined until one value is left.
+// No sort: every filter keeps a prefix of one order, so a cut (a value, and how many of
+// the tokens equal to it) describes it.  A cut is found by histograms over the distance
+// from the maximum: 1024 bins over 12 nats, then 1024 in the chosen bin, then (rarely)
+// over the values' bits, until one value is left.
 //
-// Sums decide between neighbouring tokens, and a boundary token can weigh 1e-6 of the
-// total: weights are computed in 64 bits and summed in 64-bit fixed point (2^-45 at
-// 128K tokens), which also makes every sum independent of the order of the atomics.
+// Sums decide between neighbouring tokens, and a border token can weigh 1e-6 of the
+// total: weights are computed in 64 bits and summed in fixed point (2^-45 at 128K
+// tokens), which makes every sum exact and independent of the order of the atomics.
+//
+// A row is worked on by a cluster of 1 to 8 CTAs, each holding a run of indexes, its warps
+// runs of that; they exchange totals over distributed shared memory.  Every decision
+// follows from exchanged values, so all CTAs of a cluster take the same barriers.
+#include <string.h>
+
+#include <type_traits>
+
 #include "common.cuh"
 #include "host_util.h"
 
 namespace asb {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 2048;           // two bins per thread
-constexpr int kDistBits = 22;         // distance Q: two histogram levels of 11 bits
-constexpr float kDistRange = 32.f;    // nats covered by Q before it saturates
-constexpr int kMaxVocab = 1 << 24;
+constexpr int kMaxCluster = 8;
+constexpr int kBinBits = 10;
+constexpr int kBins = 1 << kBinBits;
+constexpr float kWindow = 12.f;  // nats covered by the first histogram
+constexpr int kTable = 512;      // 2^(i / 512)
+constexpr int kMaxVocab = 1 << 20;
+typedef unsigned long long u64;
 
 __device__ __forceinline__ float sanitize(float v) {
   if (v != v) return 0.f;
   if (v == INFINITY) return 1e4f;
   if (v == -INFINITY) return -1e4f;
-  return v == 0.f ? 0.f : v;  // -0 ties with +0
+  return v;
 }
-// Order-preserving bits of an fp32 value.
+// Order-preserving bits of an fp32 value; -0 as +0.
 __device__ __forceinline__ uint32_t ord_key(float v) {
-  const uint32_t b = __float_as_uint(v);
+  const uint32_t b = __float_as_uint(v + 0.f);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
 }
 
-// Calls f(x, index) for the elements [i0, i1) of a row, 32 lanes x 16 bytes at a time.
-template <typename T, typename F>
-__device__ __forceinline__ void visit(const T* __restrict__ row, int i0, int i1, bool vec, F f) {
-  constexpr int VEC = 16 / int(sizeof(T));
-  const int lane = threadIdx.x & 31;
-  for (int base = i0 + lane * VEC; base < i1; base += 32 * VEC) {
-    if (vec && base + VEC <= i1) {
-      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(row + base));
-      const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) f(sanitize(Elem<T>::to_f32(e[j])), base + j);
-    } else {
-      for (int j = 0; j < VEC && base + j < i1; ++j)
-        f(sanitize(Elem<T>::to_f32(row[base + j])), base + j);
-    }
+// ---- the cluster's shared memory -------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t peer(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ uint32_t peer_load(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void peer_store64(uint32_t addr, u64 v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+__device__ __forceinline__ void cluster_sync(int C) {
+  if (C == 1) {
+    __syncthreads();
+  } else {
+    __syncwarp();  // the aligned form takes whole warps
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
+                 "barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
 }
 
-__device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
+struct Slot {
+  u64 a, b, c;
+};
+struct Shared {
+  double table[kTable];          // 2^(i / 512) in units of the fixed point
+  uint32_t hist[3][kBins];       // pieces of the summed measure
+  uint32_t kmin[kBins], kmax[kBins];
+  Slot slot[2][kMaxCluster];     // exchanges, in turn
+  u64 warp[kWarps];
+  u64 warp2[kWarps];
+  Slot found;
+};
+
+struct Params {
+  int64_t* out;
+  float* logprobs;
+  const float* u;
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int64_t row_stride;
+  int V, C, chunk;      // tokens, CTAs of a cluster, tokens of a CTA
+  int frac, piece;      // bits after the point of a weight, bits of a histogram piece
+};
+
+// One CTA's view of its row.
+template <typename T>
+struct Row {
+  Shared& s;
+  const T* row;
+  int C, rank, turn;  // turn: which slot buffer the next exchange uses
+  int i0, i1;         // this warp's run of indexes
+  bool vec;           // rows from 16-byte boundaries
+  bool special;       // the row holds NaN or infinities
+  float m;
+  // weights
+  double c, md;       // log2(e) / T, m
+  int frac, piece;
+  // distances from the maximum in units of a second-level bin
+  float dscale;
+
+  // f(x, index) for this warp's tokens, 32 lanes x 16 bytes at a time
+  template <typename F>
+  __device__ __forceinline__ void visit(F f) const {
+    if (special)
+      visit_as<true>(f);
+    else
+      visit_as<false>(f);
+  }
+  template <bool kSpecial, typename F>
+  __device__ __forceinline__ void visit_as(F f) const {
+    constexpr int VEC = 16 / int(sizeof(T));
+    const int lane = threadIdx.x & 31;
+    for (int base = i0 + lane * VEC; base < i1; base += 32 * VEC) {
+      if (vec && base + VEC <= i1) {
+        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(row + base));
+        const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float x = Elem<T>::to_f32(e[j]);
+          f(kSpecial ? sanitize(x) : x, base + j);
+        }
+      } else {
+        for (int j = 0; j < VEC && base + j < i1; ++j) {
+          const float x = Elem<T>::to_f32(row[base + j]);
+          f(kSpecial ? sanitize(x) : x, base + j);
+        }
+      }
+    }
+  }
+
+  // w in fixed point: 2^y, y = (x - m) log2(e) / T, as 2^(j / 512) from the table times
+  // a cubic in the rest (|rest| <= 1/1024: relative error below 1e-14).  Adding 1.5 *
+  // 2^43 rounds y to 512ths; adding 2^52 to the product rounds it to a whole number.
+  __device__ __forceinline__ u64 fixed(float x) const {
+    const uint32_t b = __float_as_uint(x);
+    // fp32 to fp64 on the integer units (zeros and denormals become values below 1e-38)
+    const double xd = __hiloint2double(int((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)),
+                                       int(b << 29));
+    const double d = xd - md;
+    const double kRound = 6755399441055744.0 / 512.0;  // 1.5 * 2^52 / 512
+    const double t = fma(d, c, kRound);
+    const int j = __double2loint(t);
+    const double whole = t - kRound;
+    const double f = fma(d, c, -whole);
+    double p = fma(f, 0.05550410866482158, 0.24022650695910072);  // ln2^3 / 6, ln2^2 / 2
+    p = fma(p, f, 0.6931471805599453);
+    p = fma(p, f, 1.0);
+    const double tab = s.table[j & (kTable - 1)];
+    const double scaled = __hiloint2double(__double2hiint(tab) + ((j >> 9) << 20), __double2loint(tab));
+    const double v = fma(scaled, p, 4503599627370496.0);  // 2^52
+    const u64 bits = u64(__double_as_longlong(v)) & 0xFFFFFFFFFFFFFull;
+    return whole > -60.0 ? bits : 0ull;  // below half a unit (and out of the exponent's range)
+  }
+  // Distance from the maximum in second-level bins, -1 outside the window.
+  __device__ __forceinline__ int dist(float x) const {
+    const float d = (m - x) * dscale;
+    return d < float(1 << (2 * kBinBits)) ? int(d) : -1;
+  }
+
+  // Slot `v` of every CTA, at every CTA.  One barrier; two buffers in turn, so a slot is
+  // rewritten only after a barrier that follows its last reads.
+  __device__ __forceinline__ const Slot* exchange(const Slot& v) {
+    Slot* buf = s.slot[turn];
+    turn ^= 1;
+    if (threadIdx.x < C) {
+      const uint32_t at = peer(&buf[rank], threadIdx.x);
+      peer_store64(at, v.a);
+      peer_store64(at + 8, v.b);
+      peer_store64(at + 16, v.c);
+    }
+    cluster_sync(C);
+    return buf;
+  }
+
+  __device__ __forceinline__ void clear() {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+      s.hist[0][i] = s.hist[1][i] = s.hist[2][i] = 0;
+      s.kmin[i] = 0xffffffffu;
+      s.kmax[i] = 0;
+    }
+    __syncthreads();
+  }
+  template <bool kCount>
+  __device__ __forceinline__ void add(int bin, u64 v) {
+    if (kCount) {
+      atomicAdd(&s.hist[0][bin], uint32_t(v));
+    } else {
+      const uint32_t mask = (1u << piece) - 1;
+      atomicAdd(&s.hist[0][bin], uint32_t(v) & mask);
+      atomicAdd(&s.hist[1][bin], uint32_t(v >> piece) & mask);
+      const uint32_t top = uint32_t(v >> (2 * piece));
+      if (top) atomicAdd(&s.hist[2][bin], top);
+    }
+  }
+
+  struct Found {
+    int bin;        // -1: the target lies beyond the histogram
+    u64 before;     // sum above the bin (or of the whole histogram)
+    uint32_t lo, hi;  // least and largest key in it, where those were kept
+  };
+  // Sums the cluster's histograms and finds the first bin at which acc + the running sum
+  // reaches the target.  The histograms may be cleared afterwards.
+  __device__ Found find(u64 acc, u64 target, bool keys) {
+    cluster_sync(C);  // every CTA's histogram is complete
+    const int S = kBins / C;  // bins of this CTA's slice
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    // thread t: bins [t * per, (t + 1) * per) of the slice
+    const int per = S > kThreads ? S / kThreads : 1;  // 1 or 2
+    u64 v[2] = {0, 0};
+    if (t * per < S) {
+      for (int e = 0; e < per; ++e) {
+        const int bin = rank * S + t * per + e;
+        for (int q = 0; q < C; ++q) {
+          if (C == 1) {
+            v[e] += s.hist[0][bin] + (u64(s.hist[1][bin]) << piece) + (u64(s.hist[2][bin]) << (2 * piece));
+          } else {
+            const uint32_t at = peer(&s.hist[0][bin], q);
+            v[e] += peer_load(at) + (u64(peer_load(at + 4 * kBins)) << piece) +
+                    (u64(peer_load(at + 8 * kBins)) << (2 * piece));
+          }
+        }
+      }
+    }
+    // running sums of the slice
+    u64 inc = v[0] + v[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 n = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += n;
+    }
+    if (lane == 31) s.warp[warp] = inc;
+    __syncthreads();
+    u64 base = 0, slice = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) base += s.warp[w];
+      slice += s.warp[w];
+    }
+    const u64 e0 = base + inc - v[0] - v[1];  // of the slice, before this thread's bins
+    const Slot* all = exchange(Slot{slice, 0, 0});
+    u64 start = acc, whole = acc;
+    for (int q = 0; q < C; ++q) {
+      if (q < rank) start += all[q].a;
+      whole += all[q].a;
+    }
+    if (whole < target) return Found{-1, whole, 0, 0};
+    // the thread whose bin it is tells every CTA
+    const u64 b0 = start + e0, b1 = b0 + v[0], b2 = b1 + v[1];
+    if (b0 < target && b2 >= target) {
+      const int e = b1 >= target ? 0 : 1;
+      const int bin = rank * S + t * per + e;
+      uint32_t lo = 0xffffffffu, hi = 0;
+      if (keys) {
+        for (int q = 0; q < C; ++q) {
+          lo = min(lo, peer_load(peer(&s.kmin[bin], q)));
+          hi = max(hi, peer_load(peer(&s.kmax[bin], q)));
+        }
+      }
+      for (int q = 0; q < C; ++q) {
+        const uint32_t at = peer(&s.found, q);
+        peer_store64(at, u64(bin));
+        peer_store64(at + 8, e ? b1 : b0);
+        peer_store64(at + 16, (u64(hi) << 32) | lo);
+      }
+    }
+    cluster_sync(C);
+    const Found f{int(s.found.a), s.found.b, uint32_t(s.found.c), uint32_t(s.found.c >> 32)};
+    __syncthreads();  // read by all before it is written again
+    return f;
+  }
+
+  struct Cut {
+    float x;    // values above it are kept, and the first ties of those equal to it
+    u64 above;  // summed measure of the values above it
+  };
+  // The cut at which the running measure reaches the target.  The first histogram (over
+  // the window) is filled; measure(x) is 0 for tokens out of the running.
+  template <bool kCount, typename M>
+  __device__ Cut select(u64 target, M measure) {
+    Found f = find(0, target, false);
+    u64 acc = f.before;
+    uint32_t lo = 0, hi = ord_key(m);
+    int q = -1;  // second-level distance of the tokens left, -1: those beyond the window
+    clear();
+    if (f.bin >= 0) {
+      const int b1 = f.bin;
+      visit([&](float x, int) {
+        const int d = dist(x);
+        if (d >= 0 && (d >> kBinBits) == b1) {
+          const u64 v = measure(x);
+          if (v) {
+            add<kCount>(d & (kBins - 1), v);
+            atomicMin(&s.kmin[d & (kBins - 1)], ord_key(x));
+            atomicMax(&s.kmax[d & (kBins - 1)], ord_key(x));
+          }
+        }
+      });
+      f = find(acc, target, true);
+      q = (b1 << kBinBits) | max(f.bin, 0);
+      acc = f.before;
+      lo = f.lo;
+      hi = f.hi;
+      clear();
+    }
+    // the tokens left differ in their lowest bits only, or lie beyond the window: by key,
+    // ten bits at a time
+    for (int level = 0; lo < hi && level < 4; ++level) {
+      int shift = 0;
+      while (((hi - lo) >> shift) >= uint32_t(kBins)) ++shift;
+      visit([&](float x, int) {
+        const uint32_t k = ord_key(x);
+        if (k < lo || k > hi || dist(x) != q) return;
+        const u64 v = measure(x);
+        if (v) add<kCount>(int((hi - k) >> shift), v);
+      });
+      f = find(acc, target, false);
+      acc = f.before;
+      const uint32_t top = hi - (uint32_t(max(f.bin, 0)) << shift);
+      const uint32_t width = (1u << shift) - 1;
+      lo = top - lo > width ? top - width : lo;
+      hi = top;
+      clear();
+    }
+    return Cut{key_value(hi), acc};
+  }
+};
+
+__device__ __forceinline__ u64 warp_sum(u64 v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-struct Shared {
-  unsigned long long hist[kBins];
-  unsigned long long warp[kWarps];
-  unsigned long long before;  // sum of everything above the chosen bin
-  uint32_t lo, hi;
-  int bin;
-};
-
-// Sum over the block; every thread gets it.
-__device__ unsigned long long block_sum(Shared& s, unsigned long long v) {
-  v = warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s.warp[threadIdx.x >> 5] = v;
-  __syncthreads();
-  unsigned long long t = 0;
-  for (int w = 0; w < kWarps; ++w) t += s.warp[w];
-  return t;
-}
-
-// First bin at which acc + (sums of bins up to it) reaches target, and the sum before it.
-__device__ void find_bin(Shared& s, unsigned long long acc, unsigned long long target) {
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  __syncthreads();
-  const unsigned long long a = s.hist[2 * t], b = s.hist[2 * t + 1];
-  unsigned long long inc = a + b;
+// Maximum of this warp's tokens (NaN ignored), and whether any is NaN or infinite.  Two
+// 16-bit elements at a time: adding one to the exponent's lowest bit carries into the
+// sign's place exactly when all its bits are set.
+template <typename T>
+__device__ __forceinline__ void scan_max(const T* row, int i0, int i1, bool vec, float& mx,
+                                         uint32_t& special) {
+  constexpr int VEC = 16 / int(sizeof(T));
+  const int lane = threadIdx.x & 31;
+  mx = -INFINITY;
+  special = 0;
+  for (int base = i0 + lane * VEC; base < i1; base += 32 * VEC) {
+    if (vec && base + VEC <= i1) {
+      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(row + base));
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+      if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long n = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += n;
+        for (int j = 0; j < 4; ++j) {
+          mx = fmaxf(mx, __uint_as_float(w[j]));
+          special |= ((w[j] & 0x7fffffffu) + 0x00800000u) & 0x80000000u;
+        }
+      } else {
+        constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
+        constexpr uint32_t kInc = kBF16 ? 0x00800080u : 0x04000400u;
+        using T2 = typename std::conditional<kBF16, __nv_bfloat162, __half2>::type;
+        T2 v[4];
+        memcpy(v, w, 16);
+        const T2 a = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+        mx = fmaxf(mx, fmaxf(Elem<T>::to_f32(a.x), Elem<T>::to_f32(a.y)));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) special |= ((w[j] & 0x7fff7fffu) + kInc) & 0x80008000u;
+      }
+    } else {
+      for (int j = 0; j < VEC && base + j < i1; ++j) {
+        const float x = Elem<T>::to_f32(row[base + j]);
+        mx = fmaxf(mx, x);
+        special |= ((__float_as_uint(x) & 0x7fffffffu) + 0x00800000u) & 0x80000000u;
+      }
+    }
   }
-  if (lane == 31) s.warp[warp] = inc;
-  if (t == 0) {
-    s.bin = 0;
-    s.before = acc;
-  }
-  __syncthreads();
-  unsigned long long base = acc;
-  for (int w = 0; w < warp; ++w) base += s.warp[w];
-  const unsigned long long e0 = base + inc - a - b;  // before bin 2t
-  if (e0 < target && e0 + a >= target) {
-    s.bin = 2 * t;
-    s.before = e0;
-  } else if (e0 + a < target && e0 + a + b >= target) {
-    s.bin = 2 * t + 1;
-    s.before = e0 + a;
-  }
-  __syncthreads();
-}
-
-// The threshold of a filter: keys above `key` are kept, and of those equal to it the
-// first `ties` in index order.
-struct Cut {
-  uint32_t key;
-  unsigned long long above;  // summed measure of the keys above it
-};
-
-// Finds the key at which the running measure (count or weight, in the descending
-// order) reaches `target`; the caller guarantees that the whole row's measure does.
-// measure(x, key) is 0 for tokens out of the running.
-template <typename T, typename M>
-__device__ Cut select_cut(Shared& s, const T* row, int i0, int i1, bool vec, float m, float dscale,
-                          unsigned long long target, M measure) {
-  auto dist = [&](float x) -> int {
-    const float y = (m - x) * dscale;
-    return y >= float((1 << kDistBits) - 1) ? (1 << kDistBits) - 1 : int(y);
-  };
-  auto clear = [&]() {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.hist[i] = 0;
-    __syncthreads();
-  };
-  unsigned long long acc = 0;
-  clear();
-  visit(row, i0, i1, vec, [&](float x, int) {
-    const unsigned long long v = measure(x, ord_key(x));
-    if (v) atomicAdd(&s.hist[dist(x) >> 11], v);
-  });
-  find_bin(s, acc, target);
-  const int b1 = s.bin;
-  acc = s.before;
-  clear();
-  visit(row, i0, i1, vec, [&](float x, int) {
-    const int q = dist(x);
-    if ((q >> 11) != b1) return;
-    const unsigned long long v = measure(x, ord_key(x));
-    if (v) atomicAdd(&s.hist[q & 2047], v);
-  });
-  find_bin(s, acc, target);
-  const int q = (b1 << 11) | s.bin;
-  acc = s.before;
-  // keys at this distance
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    s.lo = 0xffffffffu;
-    s.hi = 0;
-  }
-  __syncthreads();
-  visit(row, i0, i1, vec, [&](float x, int) {
-    if (dist(x) != q || !measure(x, ord_key(x))) return;
-    atomicMin(&s.lo, ord_key(x));
-    atomicMax(&s.hi, ord_key(x));
-  });
-  __syncthreads();
-  uint32_t lo = s.lo, hi = s.hi;
-  // a 32-bit key takes three levels of 11 bits at most (the bound also ends the loop
-  // should another stream rewrite the logits meanwhile)
-  for (int level = 0; lo < hi && level < 3; ++level) {
-    int shift = 0;
-    while (((hi - lo) >> shift) >= uint32_t(kBins)) ++shift;
-    clear();
-    visit(row, i0, i1, vec, [&](float x, int) {
-      const uint32_t k = ord_key(x);
-      if (k < lo || k > hi) return;
-      const unsigned long long v = measure(x, k);
-      if (v) atomicAdd(&s.hist[(hi - k) >> shift], v);
-    });
-    find_bin(s, acc, target);
-    acc = s.before;
-    const uint32_t top = hi - (uint32_t(s.bin) << shift);
-    const uint32_t width = (1u << shift) - 1;
-    lo = top - lo > width ? top - width : lo;
-    hi = top;
-  }
-  return Cut{hi, acc};
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-sample_tokens_kernel(int64_t* __restrict__ out, float* __restrict__ logprobs,
-                     const T* __restrict__ logits, int64_t row_stride, int V,
-                     const float* __restrict__ u, const float* __restrict__ temperature,
-                     const int32_t* __restrict__ top_k, const float* __restrict__ top_p,
-                     const float* __restrict__ min_p, int frac_bits) {
+__global__ void __launch_bounds__(kThreads, 2)
+sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
   __shared__ Shared s;
-  const int r = blockIdx.x;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const T* row = logits + int64_t(r) * row_stride;
-  const bool vec = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
-  // every warp owns one run of indexes, so sums per warp are sums in index order
-  const int chunk = ((V + kWarps - 1) / kWarps + 255) / 256 * 256;
-  const int i0 = min(V, warp * chunk), i1 = min(V, i0 + chunk);
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int r = blockIdx.x / p.C;
+  Row<T> w{s};
+  w.C = p.C;
+  w.rank = p.C > 1 ? int(cluster_rank()) : 0;
+  w.turn = 0;
+  w.row = logits + int64_t(r) * p.row_stride;
+  w.vec = (reinterpret_cast<uintptr_t>(w.row) & 15) == 0;
+  w.frac = p.frac;
+  w.piece = p.piece;
+  const int first = min(p.V, w.rank * p.chunk), last = min(p.V, first + p.chunk);
+  // every warp owns one run of the CTA's run, in steps of a warp's 512 bytes
+  const int per_warp = ((last - first + kWarps - 1) / kWarps + 255) / 256 * 256;
+  w.i0 = min(last, first + warp * per_warp);
+  w.i1 = min(last, w.i0 + per_warp);
 
-  unsigned long long best = 0;
-  visit(row, i0, i1, vec, [&](float x, int i) {
-    const unsigned long long k =
-        (static_cast<unsigned long long>(ord_key(x)) << 32) | (0xFFFFFFFFu - uint32_t(i));
-    best = k > best ? k : best;
-  });
+  for (int i = t; i < kTable; i += kThreads)
+    s.table[i] = exp2(double(i) / kTable) * double(1ull << p.frac);
+  w.clear();
+
+  // the maximum; the row's settings, as one CTA read them
+  float mx;
+  uint32_t special;
+  scan_max(w.row, w.i0, w.i1, w.vec, mx, special);
+  special = __reduce_or_sync(0xffffffffu, special);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long k = __shfl_xor_sync(0xffffffffu, best, o);
-    best = k > best ? k : best;
-  }
-  if (lane == 0) s.warp[warp] = best;
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (lane == 0) s.warp[warp] = (u64(special != 0) << 32) | ord_key(mx);
   __syncthreads();
-  for (int w = 0; w < kWarps; ++w) best = s.warp[w] > best ? s.warp[w] : best;
-  const float m = key_value(uint32_t(best >> 32));
+  Slot mine{0, 0, 0};
+  for (int i = 0; i < kWarps; ++i) {
+    mine.a = max(mine.a & 0xffffffffull, s.warp[i] & 0xffffffffull) |
+             ((mine.a | s.warp[i]) & (1ull << 32));
+  }
+  if (w.rank == 0) {
+    mine.b = (u64(__float_as_uint(p.temperature[r])) << 32) |
+             __float_as_uint(p.top_p ? p.top_p[r] : 1.f);
+    mine.c = (u64(uint32_t(p.top_k ? p.top_k[r] : 0)) << 32) |
+             __float_as_uint(p.min_p ? p.min_p[r] : 0.f);
+  }
+  const Slot* all = w.exchange(mine);
+  u64 top = 0;
+  w.special = false;
+  for (int q = 0; q < p.C; ++q) {
+    top = max(top, all[q].a & 0xffffffffull);
+    w.special |= (all[q].a >> 32) != 0;
+  }
+  const float T_ = __uint_as_float(uint32_t(all[0].b >> 32));
+  const float tp = __uint_as_float(uint32_t(all[0].b));
+  const int k = int(uint32_t(all[0].c >> 32));
+  const float mp = __uint_as_float(uint32_t(all[0].c));
+  w.m = key_value(uint32_t(top));
+  if (w.special) {  // over the sanitised values
+    float best = -INFINITY;
+    w.visit([&](float x, int) { best = fmaxf(best, x); });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+    __syncthreads();
+    if (lane == 0) s.warp[warp] = ord_key(best);
+    __syncthreads();
+    u64 key = 0;
+    for (int i = 0; i < kWarps; ++i) key = max(key, s.warp[i]);
+    all = w.exchange(Slot{key, 0, 0});
+    key = 0;
+    for (int q = 0; q < p.C; ++q) key = max(key, all[q].a);
+    w.m = key_value(uint32_t(key));
+  }
+  const float m = w.m;
+  const float u = p.u[r];  // used by one CTA alone
 
-  const float T_ = temperature[r];
-  const int k = top_k ? top_k[r] : 0;
-  const float p = top_p ? top_p[r] : 1.f;
-  const float mp = min_p ? min_p[r] : 0.f;
-  if (!(T_ > 1e-6f) || k == 1 || p <= 0.f || mp > 1.f) {  // only the first token is kept
-    if (threadIdx.x == 0) {
-      out[r] = int64_t(0xFFFFFFFFu - uint32_t(best & 0xFFFFFFFFull));
-      if (logprobs) logprobs[r] = 0.f;
+  // the least index that passes a test, over the cluster
+  auto first_index = [&](auto test) -> int {
+    uint32_t at = 0xffffffffu;
+    w.visit([&](float x, int i) {
+      if (test(x)) at = min(at, uint32_t(i));
+    });
+    at = __reduce_min_sync(0xffffffffu, at);
+    __syncthreads();
+    if (lane == 0) s.warp[warp] = at;
+    __syncthreads();
+    u64 least = 0xffffffffu;
+    for (int i = 0; i < kWarps; ++i) least = min(least, s.warp[i]);
+    const Slot* got = w.exchange(Slot{least, 0, 0});
+    for (int q = 0; q < p.C; ++q) least = min(least, got[q].a);
+    return int(least);
+  };
+  if (!(T_ > 1e-6f) || k == 1 || tp <= 0.f || mp > 1.f) {  // one token is kept: the first maximum
+    const int at = first_index([&](float x) { return x == m; });
+    if (w.rank == 0 && t == 0) {
+      p.out[r] = at;
+      if (p.logprobs) p.logprobs[r] = 0.f;
+    }
+    if (p.C > 1) cluster_sync(p.C);  // no CTA leaves while its slots may be written
+    return;
+  }
+  const double T64 = double(T_);
+  w.c = 1.4426950408889634 / T64;
+  w.md = double(m);
+  w.dscale = float(double(1 << (2 * kBinBits)) / double(kWindow) / T64);
+
+  // -FLT_MAX - 1: everything is above the cut
+  float cut = -INFINITY;
+  u64 ties = ~0ull;
+  if (k > 0 && k < p.V) {
+    w.visit([&](float x, int) {
+      const int d = w.dist(x);
+      if (d >= 0) w.template add<true>(d >> kBinBits, 1);
+    });
+    const auto c = w.template select<true>(u64(k), [](float) { return 1ull; });
+    cut = c.x;
+    ties = u64(k) - c.above;
+  }
+  if (tp < 1.f) {
+    // weights of the first n_k: all above the cut, and `ties` times the weight at it
+    u64 z = 0;
+    w.visit([&](float x, int) {
+      if (x > cut) {
+        const u64 f = w.fixed(x);
+        z += f;
+        const int d = w.dist(x);
+        if (d >= 0) w.template add<false>(d >> kBinBits, f);
+      }
+    });
+    z = warp_sum(z);
+    __syncthreads();
+    if (lane == 0) s.warp[warp] = z;
+    __syncthreads();
+    z = 0;
+    for (int i = 0; i < kWarps; ++i) z += s.warp[i];
+    all = w.exchange(Slot{z, 0, 0});
+    z = 0;
+    for (int q = 0; q < p.C; ++q) z += all[q].a;
+    const u64 above = z;
+    const u64 wcut = cut == -INFINITY ? 0 : w.fixed(cut);
+    if (cut != -INFINITY) z += ties * wcut;
+    u64 target = u64(ceil(double(z) * double(tp)));
+    if (target < 1) target = 1;
+    if (target <= above) {  // else the boundary lies among the ties at the cut
+      const float old = cut;
+      const auto c = w.template select<false>(
+          target, [&](float x) { return x > old ? w.fixed(x) : 0ull; });
+      cut = c.x;
+      const u64 wc = max(w.fixed(cut), u64(1));
+      ties = (target - c.above + wc - 1) / wc;
+    } else if (wcut > 0) {
+      ties = min(ties, (target - above + wcut - 1) / wcut);
+    }
+  }
+  if (mp > 0.f) {
+    // min-p is a threshold on the weight: the least value that passes, found by stepping
+    // from its closed form
+    auto pass = [&](float x) { return exp((double(x) - double(m)) / T64) >= double(mp); };
+    const double at = double(m) + T64 * log(double(mp));
+    if (at > -3e38) {
+      uint32_t key = ord_key(float(at));
+      for (int i = 0; i < 4 && pass(key_value(key - 1)); ++i) --key;
+      for (int i = 0; i < 8 && !pass(key_value(key)); ++i) ++key;
+      const float least = key_value(key);
+      if (least > cut) {
+        cut = least;
+        ties = ~0ull;
+      }
+    }
+  }
+  // sums of the kept tokens above the cut and the number at it, by warp and CTA
+  u64 sum = 0;
+  uint32_t n_ties = 0, lowest = 0xffffffffu;
+  w.visit([&](float x, int) {
+    if (x > cut) sum += w.fixed(x);
+    n_ties += x == cut;
+  });
+  if (!(u > 0.f))  // the first kept token of positive weight (in 64 bits: above 2^-1074)
+    w.visit([&](float x, int i) {
+      if (x >= cut && (double(x) - w.md) * w.c > -1074.0) lowest = min(lowest, uint32_t(i));
+    });
+  sum = warp_sum(sum);
+  const u64 n_tie = __reduce_add_sync(0xffffffffu, n_ties);
+  lowest = __reduce_min_sync(0xffffffffu, lowest);
+  __syncthreads();
+  if (lane == 0) {
+    s.warp[warp] = sum;
+    s.warp2[warp] = (n_tie << 32) | lowest;
+  }
+  __syncthreads();
+  Slot totals{0, 0, 0xffffffffu};
+  for (int i = 0; i < kWarps; ++i) {
+    totals.a += s.warp[i];
+    totals.b += s.warp2[i] >> 32;
+    totals.c = min(totals.c & 0xffffffffull, s.warp2[i] & 0xffffffffull);
+  }
+  if (w.rank == 0) totals.c |= u64(__float_as_uint(u)) << 32;
+  all = w.exchange(totals);
+  const float uu = __uint_as_float(uint32_t(all[0].c >> 32));
+  const u64 wcut = cut == -INFINITY ? 0 : w.fixed(cut);
+  u64 before = 0, total = 0, t_before = 0, t_all = 0, low = 0xffffffffu;
+  for (int q = 0; q < p.C; ++q) {
+    if (q < w.rank) {
+      before += all[q].a;
+      t_before += all[q].b;
+    }
+    total += all[q].a;
+    t_all += all[q].b;
+    low = min(low, all[q].c & 0xffffffffull);
+  }
+  total += min(ties, t_all) * wcut;
+  for (int i = 0; i < warp; ++i) {
+    before += s.warp[i];
+    t_before += s.warp2[i] >> 32;
+  }
+  before += min(ties, t_before) * wcut;
+  u64 quota = ties > t_before ? min(ties - t_before, n_tie) : 0;  // this warp's ties
+  const u64 here = sum + quota * wcut;
+  const double one = double(1ull << p.frac);
+  auto write = [&](int i, float x) {
+    p.out[r] = i;
+    if (p.logprobs)
+      p.logprobs[r] = float((double(x) - double(m)) / T64 - log(double(total) / one));
+  };
+  if (p.C > 1) cluster_sync(p.C);  // every CTA has read its slots: none is used from here on
+  if (!(uu > 0.f)) {
+    if (w.rank == 0 && t == 0) {
+      const float x = Elem<T>::to_f32(w.row[low]);
+      write(int(low), sanitize(x));
     }
     return;
   }
-  const double inv_t = 1.0 / double(T_);
-  const float dscale = float(double(1 << kDistBits) / double(kDistRange) * inv_t);
-  const double one = double(1ull << frac_bits);
-  auto weight = [&](float x) -> double { return exp((double(x) - double(m)) * inv_t); };
-  // a token of positive weight counts at least one unit, so u = 0 can reach it
-  auto fixed = [&](float x) -> unsigned long long {
-    const double w = weight(x);
-    const unsigned long long f = static_cast<unsigned long long>(__double2ll_rn(w * one));
-    return f == 0 && w > 0.0 ? 1 : f;
-  };
-
-  uint32_t cut = 0;  // smallest key kept; of the tokens equal to it, `ties` are
-  unsigned long long ties = ~0ull;
-  if (k > 0 && k < V) {
-    const Cut c = select_cut(s, row, i0, i1, vec, m, dscale, static_cast<unsigned long long>(k),
-                             [&](float, uint32_t) { return 1ull; });
-    cut = c.key;
-    ties = static_cast<unsigned long long>(k) - c.above;
-  }
-  if (p < 1.f) {
-    // weights of the first n_k: all above the cut, and `ties` times the weight at it
-    unsigned long long z = 0;
-    visit(row, i0, i1, vec, [&](float x, int) {
-      if (ord_key(x) > cut) z += fixed(x);
-    });
-    z = block_sum(s, z);
-    const unsigned long long wcut = cut ? fixed(key_value(cut)) : 0;
-    if (cut) z += ties * wcut;
-    const unsigned long long target =
-        static_cast<unsigned long long>(ceil(double(z) * double(p)));
-    const unsigned long long above_cut = cut ? z - ties * wcut : z;
-    if (target <= above_cut) {  // else the boundary lies among the ties at the cut
-      const Cut c = select_cut(s, row, i0, i1, vec, m, dscale, target > 0 ? target : 1,
-                               [&](float x, uint32_t key) { return key > cut ? fixed(x) : 0ull; });
-      cut = c.key;
-      const unsigned long long w = fixed(key_value(cut));
-      ties = (target - c.above + w - 1) / w;
-    } else {
-      const unsigned long long need = (target - above_cut + wcut - 1) / wcut;
-      ties = need < ties ? need : ties;
-    }
-  }
-  // min-p is a threshold on the weight alone
-  const double mpd = double(mp);
-  auto above = [&](float x) { return ord_key(x) > cut && (!(mp > 0.f) || weight(x) >= mpd); };
-  const bool cut_kept = cut != 0 && (!(mp > 0.f) || weight(key_value(cut)) >= mpd);
-  const unsigned long long wcut = cut_kept ? fixed(key_value(cut)) : 0;
-
-  // how many of the ties lie before this warp's run
-  unsigned long long tie_count = 0;
-  if (cut_kept) {
-    visit(row, i0, i1, vec, [&](float x, int) { tie_count += ord_key(x) == cut; });
-    tie_count = warp_sum(tie_count);
-  }
-  __syncthreads();
-  if (lane == 0) s.warp[warp] = tie_count;
-  __syncthreads();
-  unsigned long long ties_before = 0;
-  for (int w = 0; w < warp; ++w) ties_before += s.warp[w];
-  unsigned long long quota = ties > ties_before ? ties - ties_before : 0;
-  if (quota > tie_count) quota = tie_count;
-
-  unsigned long long sum = 0;
-  visit(row, i0, i1, vec, [&](float x, int) {
-    if (above(x)) sum += fixed(x);
-  });
-  sum = warp_sum(sum) + quota * wcut;
-  __syncthreads();
-  if (lane == 0) s.warp[warp] = sum;
-  __syncthreads();
-  unsigned long long before = 0, total = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += s.warp[w];
-    total += s.warp[w];
-  }
-  const float uu = u[r];
-  // u outside [0, 1): the first / last kept token of positive weight
-  unsigned long long target = uu > 0.f ? static_cast<unsigned long long>(double(uu) * double(total)) : 0;
+  u64 target = u64(double(uu) * double(total));
   if (target >= total) target = total - 1;
-  if (!(before <= target && target < before + sum)) return;
-  // this warp's run holds the token: walk it 32 elements at a time
-  unsigned long long c = before;
-  for (int base = i0; base < i1; base += 32) {
-    const int i = base + lane;
-    const float x = i < i1 ? sanitize(Elem<T>::to_f32(row[i])) : 0.f;
-    const bool in = i < i1;
-    const bool tie = in && cut_kept && ord_key(x) == cut;
-    const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie);
-    const bool kept = in && (above(x) || (tie && __popc(tie_mask & ((1u << lane) - 1)) < quota));
-    unsigned long long w = kept ? fixed(x) : 0;
-    unsigned long long inc = w;
+  if (!(before <= target && target < before + here)) return;
+  // this warp's run holds the token: 32 lanes x 8 tokens at a time
+  constexpr int kStep = 8;
+  u64 c = before;
+  for (int base = w.i0; base < w.i1; base += 32 * kStep) {
+    const int i0 = base + lane * kStep;
+    float x[kStep];
+    uint32_t my_ties = 0;
+#pragma unroll
+    for (int j = 0; j < kStep; ++j) {
+      x[j] = i0 + j < w.i1 ? sanitize(Elem<T>::to_f32(w.row[i0 + j])) : -INFINITY;
+      my_ties += i0 + j < w.i1 && x[j] == cut;
+    }
+    uint32_t ties_inc = my_ties;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long n = __shfl_up_sync(0xffffffffu, inc, o);
+      const uint32_t n = __shfl_up_sync(0xffffffffu, ties_inc, o);
+      if (lane >= o) ties_inc += n;
+    }
+    uint32_t tie = ties_inc - my_ties;  // ties before this lane's tokens
+    u64 v[kStep], mine_sum = 0;
+#pragma unroll
+    for (int j = 0; j < kStep; ++j) {
+      v[j] = 0;
+      if (i0 + j < w.i1) {
+        if (x[j] > cut)
+          v[j] = w.fixed(x[j]);
+        else if (x[j] == cut && u64(tie++) < quota)
+          v[j] = wcut;
+      }
+      mine_sum += v[j];
+    }
+    u64 inc = mine_sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 n = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += n;
     }
     const uint32_t hit = __ballot_sync(0xffffffffu, c + inc > target);
     if (hit) {
       if (lane == __ffs(hit) - 1) {
-        out[r] = i;
-        if (logprobs) logprobs[r] = float((double(x) - double(m)) * inv_t - log(double(total) / one));
+        u64 run = c + inc - mine_sum;
+        int at = 0;
+#pragma unroll
+        for (int j = 0; j < kStep; ++j) {
+          run += v[j];
+          if (run <= target) at = j + 1;
+        }
+        write(i0 + at, sanitize(Elem<T>::to_f32(w.row[i0 + at])));
       }
       return;
     }
     c += __shfl_sync(0xffffffffu, inc, 31);
-    const uint32_t n_tie = __popc(tie_mask);
-    quota -= quota < n_tie ? quota : n_tie;
+    const u64 used = __shfl_sync(0xffffffffu, ties_inc, 31);
+    quota -= min(quota, used);
   }
+}
+
+// CTAs of a row's cluster: enough to fill the SMs (two CTAs each) when rows are few, at
+// least 2048 tokens each so that the exchanges do not outweigh the work, and never more
+// than 2^17 tokens each (the histogram pieces' range).
+int cluster_size(int rows, int vocab) {
+  int c = 1;
+  while (c < kMaxCluster &&
+         ((int64_t(rows) * c * 2 <= 2 * int64_t(sm_count()) && vocab / (2 * c) >= 2048) ||
+          (vocab + c - 1) / c > (1 << 17)))
+    c *= 2;
+  return c;
 }
 
 }  // namespace
@@ -362,21 +717,51 @@ extern "C" int as_sample_tokens(int64_t* out, float* logprobs, const void* logit
     return fail(AS_ERR_INVALID_ARG, "as_sample_tokens: bad sizes");
   if (vocab > kMaxVocab)
     return fail(AS_ERR_UNSUPPORTED, "as_sample_tokens: vocab > %d", kMaxVocab);
+  if (num_rows > (1 << 24)) return fail(AS_ERR_INVALID_ARG, "as_sample_tokens: too many rows");
   if (num_rows == 0) return AS_OK;
   if (!out || !logits || !u || !temperature)
     return fail(AS_ERR_INVALID_ARG, "as_sample_tokens: null pointer");
   if (reinterpret_cast<uintptr_t>(logits) % dtype_size(dtype))
     return fail(AS_ERR_INVALID_ARG, "as_sample_tokens: logits are not aligned to their type");
-  // the sum of `vocab` weights of at most 1 stays below 2^62
-  int bits = 0;
-  while ((1 << bits) < vocab) ++bits;
-  const int frac = 62 - bits;
+  Params p{};
+  p.out = out;
+  p.logprobs = logprobs;
+  p.u = u;
+  p.temperature = temperature;
+  p.top_k = top_k;
+  p.top_p = top_p;
+  p.min_p = min_p;
+  p.row_stride = row_stride;
+  p.V = vocab;
+  p.C = cluster_size(num_rows, vocab);
+  p.chunk = ((vocab + p.C - 1) / p.C + 255) / 256 * 256;
+  // a histogram piece of a CTA's tokens stays below 2^32, the sum of all weights (at
+  // most 1 each) below 2^62
+  const auto log2_up = [](int n) {
+    int b = 0;
+    while ((int64_t(1) << b) < n) ++b;
+    return b;
+  };
+  p.piece = 32 - log2_up(p.chunk);
+  if (p.piece > 20) p.piece = 20;
+  p.frac = 45;
+  if (p.frac > 3 * p.piece - 1) p.frac = 3 * p.piece - 1;
+  if (p.frac > 62 - log2_up(vocab)) p.frac = 62 - log2_up(vocab);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   auto run = [&](auto tag) -> int {
     using T = decltype(tag);
-    sample_tokens_kernel<T><<<num_rows, kThreads, 0, s>>>(
-        out, logprobs, static_cast<const T*>(logits), row_stride, vocab, u, temperature, top_k,
-        top_p, min_p, frac);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(num_rows) * p.C);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.C;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.C > 1 ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T>, static_cast<const T*>(logits), p);
     return check_launch("as_sample_tokens");
   };
   switch (dtype) {

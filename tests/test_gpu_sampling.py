@@ -138,6 +138,25 @@ def test_sample_extreme_settings():
     check(x, [0.0, 1.0, -1.0, 2.0, 0.99999994, 0.0, 1.0], [0.9] * 7, p=[0.95] * 7)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("B,V", [(2, 30011), (3, 4096), (200, 2500)])
+def test_sample_small_and_large_values(B, V, dtype):
+    """Logits all next to zero, on both sides of it, large, and far apart: cuts among
+    values of every size."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    n = torch.randn(B, V, generator=g, device=DEV)
+    u = torch.rand(B, generator=torch.Generator().manual_seed(B)).tolist()
+    for x in (n * 1e-3, n * 1e-5, n * 0.02, n * 3e-39, n * 40.0, n.abs() * 200.0, -n.abs() * 300.0,
+              -n.abs() * 0.01, torch.where(n > 0, n * 1e-4, n * 8.0),
+              torch.where(n > 1.5, 0.0, -500.0) + 0 * n, torch.where(n > 0, 0.0, -0.0)):
+        x = x.to(dtype)
+        check(x, u, [0.7] * B, p=[0.6] * B)
+        check(x, u, [1.1] * B, k=[V // 3] * B, p=[0.97] * B, mp=[0.001] * B)
+        check(x, u, [0.05] * B, k=[V // 2] * B)
+        if B < 100:
+            check(x, u, [60.0] * B, p=[0.5] * B)
+
+
 def test_sample_u_zero_skips_nothing_of_positive_weight():
     """u = 0 takes the first kept token however unlikely, but none of weight 0."""
     x = torch.tensor([[-60.0, 0.0, 3.0], [-900.0, 0.0, 3.0]], device=DEV)

@@ -21,6 +21,7 @@
 // A row is worked on by a cluster of 1 to 8 CTAs, each holding a run of indexes, its warps
 // runs of that; they exchange totals over distributed shared memory.  Every decision
 // follows from exchanged values, so all CTAs of a cluster take the same barriers.
+#include <stddef.h>
 #include <string.h>
 
 #include <type_traits>
@@ -113,31 +114,46 @@ struct Queue {
 };
 
 // bf16 rows: a histogram by value.  The 4096 values of magnitude 2^-9 to 128 have a
-// bin each, in descending order; the few closer to zero are listed; those at or below
-// -128 (masks) weigh nothing next to any maximum this path accepts.  The first pass then
-// needs no maximum and no exponential, both cuts come from one merge, and the second
-// pass looks the weights up.  Rows outside this (values of 128 and more, NaN, cuts among
-// the listed values, u <= 0) take the general path.
+// bin each; the few closer to zero are listed; those at or below -128 (masks) weigh
+// nothing next to any maximum this path accepts.  The first pass then needs no maximum
+// and no exponential, both cuts come from one merge, and the second pass looks the
+// weights up.  Rows outside this (values of 128 and more, NaN, cuts among the listed
+// values, u <= 0) take the general path.
+//
+// The passes are bound by integer instructions (half rate), so a value's place is two
+// logic operations and a multiply-add away from its 16 bits: counts (4 bytes each) and
+// weights (8) lie in ascending magnitude, those of the negative values 0x8000 bytes after
+// those of the positive ones.
 constexpr int kValueLo = (127 - 9) << 7;  // bits of 2^-9
 constexpr int kValues = 16 << 7;          // values of one sign
 constexpr int kListed = 2048;
 struct ByValue {
-  u64 weight[2 * kValues];
-  uint32_t count[2 * kValues];
+  uint32_t positive[kValues];      // counts
+  u64 weight_positive[kValues];
   uint16_t list[kListed];
-  uint32_t n_listed, refuse;
+  uint32_t n_listed, refuse, pad[(0x8000 - 28 * 1024) / 4 - 2];
+  uint32_t negative[kValues];      // byte 0x8000
+  u64 weight_negative[kValues];
 };
-// Bin of a token's value; at or above 2 * kValues for one without a bin.
-__device__ __forceinline__ uint32_t value_bin(float x) {
-  const uint32_t b = __float_as_uint(x);
-  const uint32_t d = ((b >> 16) & 0x7fff) - kValueLo;
-  return d < uint32_t(kValues) ? d ^ ((b >> 31) ? kValues : kValues - 1) : 0x80000000u;
+static_assert(offsetof(ByValue, negative) - offsetof(ByValue, positive) == 0x8000 &&
+                  offsetof(ByValue, weight_negative) - offsetof(ByValue, weight_positive) == 0x8000,
+              "layout");
+__device__ __forceinline__ bool has_bin(uint32_t code) {
+  return (code & 0x7fff) - uint32_t(kValueLo) < uint32_t(kValues);
 }
-__device__ __forceinline__ float bin_value(int bin) {
-  const uint32_t code = bin < kValues ? uint32_t(kValueLo + kValues - 1 - bin)
-                                      : 0x8000u | uint32_t(kValueLo + bin - kValues);
-  return __uint_as_float(code << 16);
+// Byte offsets of a value's count and weight from the (virtual) ones of +0.
+__device__ __forceinline__ uint32_t count_offset(uint32_t code) {
+  return (code & 0x7fff) * 4 + (code & 0x8000);
 }
+__device__ __forceinline__ uint32_t weight_offset(uint32_t code) {
+  return (code & 0x7fff) * 8 + (code & 0x8000);
+}
+// Values in descending order: bin -> code.
+__device__ __forceinline__ uint32_t bin_code(int bin) {
+  return bin < kValues ? uint32_t(kValueLo + kValues - 1 - bin)
+                       : 0x8000u | uint32_t(kValueLo + bin - kValues);
+}
+__device__ __forceinline__ float code_value(uint32_t code) { return __uint_as_float(code << 16); }
 
 struct Params {
   int64_t* out;
@@ -192,7 +208,7 @@ struct Row {
   Shared* sp;
   const T* row;
   Queue* queue;
-  const u64* by_value;  // weights by value (bf16), or null
+  const ByValue* by_value;  // weights by value (bf16), or null
   int C, rank, turn;    // turn: which slot buffer the next exchange uses
   int i0, i1;           // this warp's run of indexes
   bool vec;             // the row starts at a 16-byte boundary
@@ -264,6 +280,17 @@ struct Row {
     const u64 bits = u64(__double_as_longlong(v)) & 0xFFFFFFFFFFFFFull;
     return whole > -60.0 ? bits : 0ull;  // below half a unit (and out of the exponent's range)
   }
+  // The weight of a token, looked up where the row has a table.
+  __device__ __forceinline__ u64 weight(float x) const {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const uint32_t code = __float_as_uint(x) >> 16;
+      if (by_value && has_bin(code))
+        return *reinterpret_cast<const u64*>(
+            reinterpret_cast<const uint8_t*>(by_value->weight_positive) +
+            (weight_offset(code) - 8 * kValueLo));
+    }
+    return fixed(x);
+  }
   // Distance from the maximum in second-level bins, -1 outside the window.
   __device__ __forceinline__ int dist(float x) const {
     const float d = (m - x) * dscale;
@@ -300,6 +327,16 @@ struct Row {
     if (top) atomicAdd(&sp->hist[2][bin], top);
   }
 };
+
+// A weight outside the passes, where the code's size counts more than a call.
+template <typename T>
+__device__ __noinline__ u64 fixed_call(const Shared* sp, double md, double c, float x) {
+  Row<T> w;
+  w.sp = const_cast<Shared*>(sp);
+  w.md = md;
+  w.c = c;
+  return w.fixed(x);
+}
 
 // Sums the cluster's histograms and finds the first bin at which acc + the running sum
 // reaches the target, by way of one exchange.  The histograms may be cleared afterwards.
@@ -489,72 +526,137 @@ __device__ __noinline__ Kept sum_above(Row<T> w, float cut, bool hist) {
   return Kept{warp_sum(sum), __reduce_add_sync(0xffffffffu, ties)};
 }
 
-// The same for a bf16 row with weights by value.
-__device__ __forceinline__ Kept sum_above_by_value(const Row<__nv_bfloat16>& w, float cut) {
-  constexpr int VEC = 8;
+__device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t w) {
+  __nv_bfloat162 v;
+  memcpy(&v, &w, 4);
+  return v;
+}
+// Whether a pair of values has one without a bin: bits 15 and 31.
+__device__ __forceinline__ uint32_t unbinned(uint32_t w) {
+  const uint32_t mag = w & 0x7fff7fffu;
+  constexpr uint32_t kOver = 0x8000 - kValueLo - kValues, kUnder = 0x8000 - kValueLo;
+  return ((mag + kOver * 0x10001u) | ~(mag + kUnder * 0x10001u)) & 0x80008000u;
+}
+
+// f(16 bytes, index of the first token) for a warp's run of a bf16 row, undecoded, loads
+// three groups ahead; places past the run hold -infinity.  Plain arguments, so that
+// nothing of the loop lives in memory.
+template <typename F>
+__device__ __forceinline__ void visit_bf16(const uint16_t* row, int i0, int i1, bool vec, F f) {
+  const int first = i0 + int(threadIdx.x & 31) * 8;
+  const int full = vec ? (i1 - i0) / 256 : 0, groups = (i1 - i0 + 255) / 256;
+  const uint4* src = reinterpret_cast<const uint4*>(row + first);
+  const auto load = [&](int g) -> uint4 {
+    return g < full ? __ldg(src + g * 32) : make_uint4(0, 0, 0, 0);
+  };
+  uint4 r0 = load(0), r1 = load(1), r2 = load(2);
+#pragma unroll 1
+  for (int g = 0; g < full; ++g) {
+    const uint4 raw = r0;
+    r0 = r1;
+    r1 = r2;
+    r2 = load(g + 3);
+    f(raw, first + g * 256);
+  }
+#pragma unroll 1
+  for (int g = full; g < groups; ++g) {
+    uint32_t w[4] = {0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
+    const int i = first + g * 256;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i + j < i1)
+        w[j >> 1] = __byte_perm(w[j >> 1], row[i + j], j & 1 ? 0x5410 : 0x3254);
+    f(make_uint4(w[0], w[1], w[2], w[3]), i);
+  }
+}
+
+// sum_above() for a bf16 row with weights by value.
+__device__ __noinline__ Kept sum_above_by_value(Row<__nv_bfloat16> w, float cut) {
+  const __nv_bfloat162 cut2 = __float2bfloat162_rn(cut);  // exact: a bf16 value or a bound on them
+  const uint8_t* weights =
+      reinterpret_cast<const uint8_t*>(w.by_value->weight_positive) - 8 * kValueLo;
   u64 sum = 0;
   uint32_t ties = 0;
-  w.visit([&](const float(&x)[VEC], int) {
-    bool any = false;
+  visit_bf16(reinterpret_cast<const uint16_t*>(w.row), w.i0, w.i1, w.vec,
+             [&](const uint4& raw, int) {
+    const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
+    const __nv_bfloat162 top = __hmax2(__hmax2(as_bf162(word[0]), as_bf162(word[1])),
+                                       __hmax2(as_bf162(word[2]), as_bf162(word[3])));
+    if (!__any_sync(0xffffffffu, __hge2_mask(top, cut2) != 0)) return;
+    uint32_t slow = 0;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      any |= x[j] > cut;
-      ties += x[j] == cut;
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t bad = unbinned(word[j]);
+      uint32_t up = __hgt2_mask(as_bf162(word[j]), cut2);
+      ties += __popc(__heq2_mask(as_bf162(word[j]), cut2) & 0x10001u);
+      slow |= bad & up;
+      up &= ~bad;
+      if (up & 0x8000)
+        sum += *reinterpret_cast<const u64*>(weights + weight_offset(word[j]));
+      if (int(up) < 0)
+        sum += *reinterpret_cast<const u64*>(weights + weight_offset(word[j] >> 16));
     }
-    if (!__any_sync(0xffffffffu, any)) return;
-    uint32_t slow = 0;  // without a bin
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const uint32_t bin = value_bin(x[j]);
-      const bool up = x[j] > cut, has = bin < uint32_t(2 * kValues);
-      const u64 v = w.by_value[has ? bin : 0];
-      sum += up && has ? v : 0;
-      slow |= uint32_t(up && !has) << j;
-    }
-    while (slow) {
-      const int j = __ffs(slow) - 1;
-      slow &= slow - 1;
-      float y = x[0];
-#pragma unroll
-      for (int e = 1; e < VEC; ++e) y = e == j ? x[e] : y;
-      sum += w.fixed(y);
+    if (slow) {  // closer to zero than the bins (or far below: no weight)
+      uint32_t a = word[0], b = word[1], c = word[2], d = word[3];
+#pragma unroll 1
+      for (int j = 0; j < 8; ++j) {
+        const float x = code_value(a & 0xffff);
+        if (!has_bin(a) && x > cut) sum += w.fixed(x);
+        a = __funnelshift_r(a, b, 16);
+        b = __funnelshift_r(b, c, 16);
+        c = __funnelshift_r(c, d, 16);
+        d >>= 16;
+      }
     }
   });
   return Kept{warp_sum(sum), __reduce_add_sync(0xffffffffu, ties)};
 }
 
 // First pass of a bf16 row: counts by value, and the maximum.
-__device__ __forceinline__ float count_values(const Row<__nv_bfloat16>& w, ByValue& bv) {
-  constexpr int VEC = 8;
-  float mx = -INFINITY;
-  w.visit([&](const float(&x)[VEC], int i) {
-    uint32_t slow = 0;
+__device__ __noinline__ float count_values(const uint16_t* row, int i0, int i1, bool vec,
+                                           ByValue& bv) {
+  uint8_t* counts = reinterpret_cast<uint8_t*>(bv.positive) - 4 * kValueLo;
+  const auto count = [&](uint32_t code) {
+    atomicAdd(reinterpret_cast<uint32_t*>(counts + count_offset(code)), 1u);
+  };
+  __nv_bfloat162 top = __float2bfloat162_rn(-INFINITY);
+  visit_bf16(row, i0, i1, vec, [&](const uint4& raw, int) {
+    const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
+    const uint32_t odd =
+        unbinned(word[0]) | unbinned(word[1]) | unbinned(word[2]) | unbinned(word[3]);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      mx = fmaxf(mx, x[j]);
-      const uint32_t bin = value_bin(x[j]);
-      if (bin < uint32_t(2 * kValues)) atomicAdd(&bv.count[bin], 1u);
-      slow |= (bin >> 31) << j;
+    for (int j = 0; j < 4; ++j) top = __hmax2(top, as_bf162(word[j]));
+    if (!odd) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        count(word[j]);
+        count(word[j] >> 16);
+      }
+      return;
     }
-    while (slow) {
-      const int j = __ffs(slow) - 1;
-      slow &= slow - 1;
-      if (i + j >= w.i1) break;
-      float y = x[0];
-#pragma unroll
-      for (int e = 1; e < VEC; ++e) y = e == j ? x[e] : y;
-      if (fabsf(y) < 1.f) {  // closer to zero than the bins
+    // few groups: token by token
+    uint32_t a = word[0], b = word[1], c = word[2], d = word[3];
+#pragma unroll 1
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t mag = a & 0x7fff;
+      if (mag - uint32_t(kValueLo) < uint32_t(kValues)) {
+        count(a);
+      } else if (mag < uint32_t(kValueLo)) {
         const uint32_t at = atomicAdd(&bv.n_listed, 1u);
         if (at < kListed)
-          bv.list[at] = uint16_t(__float_as_uint(y) >> 16);
+          bv.list[at] = uint16_t(a);
         else
           bv.refuse = 1;
-      } else if (!(y < 0.f)) {  // 128 and more, NaN
+      } else if (!(a & 0x8000) || mag > 0x7f80) {  // 128 and more, NaN
         bv.refuse = 1;
       }
+      a = __funnelshift_r(a, b, 16);
+      b = __funnelshift_r(b, c, 16);
+      c = __funnelshift_r(c, d, 16);
+      d >>= 16;
     }
   });
-  return mx;
+  return fmaxf(__bfloat162float(top.x), __bfloat162float(top.y));
 }
 
 // Both cuts of a bf16 row from the cluster's counts by value.  cut.turn < 0: one of them
@@ -571,33 +673,40 @@ __device__ __noinline__ Cuts value_cuts(Row<__nv_bfloat16> w, ByValue& bv, int k
   constexpr int kAll = 2 * kValues, S = kAll / C, kPer = S / kThreads;  // 8, 4, 2 or 1
   // thread t: bins [rank * S + t * kPer, + kPer) summed over the cluster
   const int first = w.rank * S + t * kPer;
+  const int step = first < kValues ? -1 : 1;  // from one bin's count to the next's
+  const uint8_t* counts = reinterpret_cast<const uint8_t*>(bv.positive) - 4 * kValueLo;
+  const auto weight_of = [&](int bin) -> u64& {
+    return *reinterpret_cast<u64*>(reinterpret_cast<uint8_t*>(bv.weight_positive) - 8 * kValueLo +
+                                   weight_offset(bin_code(bin)));
+  };
   uint32_t n[kPer];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) n[e] = 0;
   uint32_t h[C][kPer];
 #pragma unroll
   for (int q = 0; q < C; ++q) {
-    const uint32_t from = peer_addr(smem_u32(&bv.count[first]), q);
+    const uint32_t from = peer_addr(smem_u32(counts + count_offset(bin_code(first))), q);
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) h[q][e] = peer_load(from + 4 * e);
+    for (int e = 0; e < kPer; ++e) h[q][e] = peer_load(from + 4 * step * e);
   }
-#pragma unroll 4
-  for (int i = t; i < kAll; i += kThreads) bv.weight[i] = w.fixed(bin_value(i));
-  u64 listed = 0;
+  u64 wt[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) wt[e] = w.fixed(code_value(bin_code(first + e)));
   for (int i = t; i < int(bv.n_listed); i += kThreads)
-    listed += w.fixed(__uint_as_float(uint32_t(bv.list[i]) << 16));
+    w.add(0, w.fixed(code_value(bv.list[i])));
 #pragma unroll
   for (int q = 0; q < C; ++q)
 #pragma unroll
     for (int e = 0; e < kPer; ++e) n[e] += h[q][e];
-  listed = block_scan(s, listed).total;  // (its barriers: the weights are there)
+  __syncthreads();  // the listed values' sum is there
+  const u64 listed = s.hist[0][0] + (u64(s.hist[1][0]) << kPiece) + (u64(s.hist[2][0]) << (2 * kPiece));
   u64 mass = 0, num = 0;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
-    if (n[e]) mass += n[e] * bv.weight[first + e];
+    if (n[e]) mass += n[e] * wt[e];
     num += n[e];
   }
-  const Scan ms = block_scan(s, mass), ns = block_scan(s, num);
+  const Scan ms = block_scan(s, mass), ns = k > 0 ? block_scan(s, num) : Scan{0, 0};
   u64 m_before = ms.before, n_before = ns.before;
   if (C == 1 && t == kThreads / 2) s.found2 = Slot{0, m_before, n_before};  // the positive values
   const Slot* all = w.exchange(Slot{ms.total, (ns.total << 32) | bv.n_listed, listed});
@@ -637,9 +746,13 @@ __device__ __noinline__ Cuts value_cuts(Row<__nv_bfloat16> w, ByValue& bv, int k
 #pragma unroll 1
     for (int e = 0; e < kPer; ++e) {
       uint32_t ne = n[0];
+      u64 we = wt[0];
 #pragma unroll
-      for (int y = 1; y < kPer; ++y) ne = y == e ? n[y] : ne;
-      const u64 da = ne ? ne * bv.weight[first + e] : 0;
+      for (int y = 1; y < kPer; ++y) {
+        ne = y == e ? n[y] : ne;
+        we = y == e ? wt[y] : we;
+      }
+      const u64 da = ne ? ne * we : 0;
       const u64 run = count ? b : a, step = count ? ne : da;
       if (run < target && run + step >= target) {
         for (int q = 0; q < C; ++q) {
@@ -656,13 +769,15 @@ __device__ __noinline__ Cuts value_cuts(Row<__nv_bfloat16> w, ByValue& bv, int k
     return place;
   };
   Cuts r{-INFINITY, ~0ull, w.turn};
+  int last = kAll - 1;  // the lowest kept value's bin
   u64 z = m_all, above = m_all, wcut = 0;
   if (k > 0 && u64(k) < n_all) {
     if (u64(k) > n_pos && u64(k) <= n_pos + n_list) return Cuts{0.f, 0, -1 - w.turn};
     const Slot f = locate(true, u64(k), s.found);
-    r.x = bin_value(int(f.a));
+    r.x = code_value(bin_code(int(f.a)));
     r.ties = u64(k) - f.c;
-    wcut = bv.weight[f.a];
+    last = int(f.a);
+    wcut = w.fixed(r.x);
     above = f.b;
     z = above + r.ties * wcut;
   }
@@ -672,13 +787,18 @@ __device__ __noinline__ Cuts value_cuts(Row<__nv_bfloat16> w, ByValue& bv, int k
     if (target <= above) {
       if (target > m_pos && target <= m_pos + m_list) return Cuts{0.f, 0, -1 - w.turn};
       const Slot f = locate(false, target, s.found2);
-      r.x = bin_value(int(f.a));
-      const u64 wc = max(bv.weight[f.a], u64(1));
+      r.x = code_value(bin_code(int(f.a)));
+      last = int(f.a);
+      const u64 wc = max(w.fixed(r.x), u64(1));
       r.ties = (target - f.b + wc - 1) / wc;
     } else if (wcut > 0) {
       r.ties = min(r.ties, (target - above + wcut - 1) / wcut);
     }
   }
+  // the kept values' weights, for the second pass
+#pragma unroll 2
+  for (int i = t; i <= last; i += kThreads) weight_of(i) = w.fixed(code_value(bin_code(i)));
+  __syncthreads();
   return r;
 }
 
@@ -724,12 +844,23 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
   for (int i = t; i < kTable; i += kThreads)
     s.table[i] = exp2(double(i) / kTable) * double(1ull << kFrac);
   if constexpr (kByValue) {
-    for (int i = t; i < 2 * kValues; i += kThreads) bv.count[i] = 0;
+    for (int i = t; i < kValues; i += kThreads) bv.positive[i] = bv.negative[i] = 0;
     if (t == 0) bv.n_listed = bv.refuse = 0;
   }
   w.clear();
   pdl_wait();  // programmatic launch: the logits come from the kernel before
   pdl_trigger();
+
+  // This CTA's run on its way to L2 at once: the passes' own loads are too few in flight
+  // to stream it from HBM.  (Whole 16-byte words of the run, 4 KB to a thread.)
+  {
+    const uintptr_t lo = (reinterpret_cast<uintptr_t>(w.row + first) + 15) & ~uintptr_t(15);
+    const uintptr_t hi = reinterpret_cast<uintptr_t>(w.row + last) & ~uintptr_t(15);
+    for (uintptr_t a = lo + uintptr_t(t) * 4096; a < hi; a += kThreads * 4096) {
+      const uint32_t bytes = uint32_t(min(hi - a, uintptr_t(4096)));
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a), "r"(bytes) : "memory");
+    }
+  }
 
   // the row's settings, as one CTA reads them
   Slot mine{0, 0, 0};
@@ -743,7 +874,7 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
   float mx = -INFINITY;
   uint32_t special = 0;
   if constexpr (kByValue) {
-    mx = count_values(w, bv);
+    mx = count_values(reinterpret_cast<const uint16_t*>(w.row), w.i0, w.i1, w.vec, bv);
   } else {
     w.visit([&](const float(&x)[VEC], int i) {
 #pragma unroll
@@ -835,13 +966,14 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
                                 : value_cuts<8>(w, bv, k, tp);
       if (c.turn >= 0) {
         w.turn = c.turn;
-        w.by_value = bv.weight;
+        w.by_value = &bv;
         cut = c.x;
         ties = c.ties;
         found = true;
       } else {
         w.turn = -1 - c.turn;
         cluster_sync(p.C);  // no peer reads the counts any more: the queue lies over them
+        w.clear();
       }
     }
   }
@@ -881,7 +1013,11 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
     }
   }
   if (mp > 0.f) {
-    const float least = least_kept(m, T64, double(mp));
+    float least = least_kept(m, T64, double(mp));
+    if (kByValue && w.by_value) {  // up to a bf16 value: the second pass compares in bf16
+      const uint32_t b = __float_as_uint(least);
+      if (b & 0xffff) least = __uint_as_float((b & 0xffff0000u) + ((b >> 31) ? 0 : 0x10000u));
+    }
     if (least > cut) {
       cut = least;
       ties = ~0ull;
@@ -907,11 +1043,7 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
   }
   all = w.exchange(Slot{ws.total, wt.total, (u64(__float_as_uint(u)) << 32) | low});
   const float uu = __uint_as_float(uint32_t(all[0].c >> 32));
-  u64 wcut = 0;
-  if (cut != -INFINITY) {
-    const uint32_t bin = kByValue && w.by_value ? value_bin(cut) : 0x80000000u;
-    wcut = bin < uint32_t(2 * kValues) ? w.by_value[bin] : w.fixed(cut);
-  }
+  const u64 wcut = cut == -INFINITY ? 0 : w.weight(cut);
   u64 before = 0, total = 0, t_before = 0, t_all = 0;
   for (int q = 0; q < p.C; ++q) {
     if (q < w.rank) {
@@ -941,8 +1073,63 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
   }
   u64 target = u64(double(uu) * double(total));
   if (target >= total) target = total - 1;
-  // The warp whose run holds the token hands the run to the whole CTA, a few tokens per
-  // thread.
+  const auto weight = [&](float x) -> u64 {  // of a token above the cut
+    if constexpr (kByValue) {
+      const uint32_t code = __float_as_uint(x) >> 16;
+      if (w.by_value && has_bin(code))
+        return *reinterpret_cast<const u64*>(
+            reinterpret_cast<const uint8_t*>(w.by_value->weight_positive) +
+            (weight_offset(code) - 8 * kValueLo));
+    }
+    return fixed_call<T>(&s, w.md, w.c, x);
+  };
+  const auto at = [&](u64 above, u64 t_seen) { return above + min(ties, t_seen) * wcut; };
+  // the token among this thread's [j0, j1), which begin after `before` and `t_before`
+  const auto pick = [&](int j0, int j1) {
+#pragma unroll 1
+    for (int i = j0; i < j1; ++i) {
+      const float x = sanitize(Elem<T>::to_f32(w.row[i]));
+      t_before += x == cut;
+      if (x > cut) before += weight(x);
+      if (at(before, t_before) > target) {
+        write(i, x);
+        return;
+      }
+    }
+  };
+  if (per_warp <= 2048) {
+    // a short run: the warp whose it is walks it, 32 lanes x 16 bytes at a time
+    if (!__shfl_sync(0xffffffffu, ahead <= target && target < after, 0)) return;
+    before = __shfl_sync(0xffffffffu, before, 0);
+    t_before = __shfl_sync(0xffffffffu, t_before, 0);
+    bool done = false;
+    w.visit([&](const float(&x)[VEC], int i) {
+      if (done) return;
+      u64 sum = 0;
+      uint32_t n = 0;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        n += x[j] == cut;
+        if (x[j] > cut) sum += weight(x[j]);
+      }
+      const u64 s_inc = warp_scan(sum), n_inc = warp_scan(n);
+      const uint32_t hit =
+          __ballot_sync(0xffffffffu, at(before + s_inc, t_before + n_inc) > target);
+      if (hit) {
+        done = true;
+        if (lane == __ffs(hit) - 1) {
+          before += s_inc - sum;
+          t_before += n_inc - n;
+          pick(i, min(i + VEC, w.i1));
+        }
+      } else {
+        before += __shfl_sync(0xffffffffu, s_inc, 31);
+        t_before += __shfl_sync(0xffffffffu, n_inc, 31);
+      }
+    });
+    return;
+  }
+  // A long one goes to the whole CTA, a few tokens per thread.
   if (lane == 0 && ahead <= target && target < after) {
     s.found = Slot{before, t_before, (u64(uint32_t(w.i0)) << 32) | uint32_t(w.i1)};
     s.flag = 1;
@@ -952,38 +1139,156 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
   before = s.found.a;
   t_before = s.found.b;
   const int run0 = int(s.found.c >> 32), run1 = int(uint32_t(s.found.c));
-  const int share = (run1 - run0 + kThreads - 1) / kThreads;
+  const int share = ((run1 - run0 + kThreads - 1) / kThreads + VEC - 1) / VEC * VEC;
   const int j0 = min(run1, run0 + t * share), j1 = min(run1, j0 + share);
-  const auto token = [&](int i) { return sanitize(Elem<T>::to_f32(w.row[i])); };
-  const auto weight = [&](float x) -> u64 {
-    if (x <= cut) return 0;
-    const uint32_t bin = kByValue && w.by_value ? value_bin(x) : 0x80000000u;
-    return bin < uint32_t(2 * kValues) ? w.by_value[bin] : w.fixed(x);
-  };
   u64 sum = 0, n_ties = 0;
 #pragma unroll 1
-  for (int i = j0; i < j1; ++i) {
-    const float x = token(i);
-    n_ties += x == cut;
-    sum += weight(x);
+  for (int i = j0; i < j1; i += VEC) {
+    T e[VEC];
+    if (w.vec && i + VEC <= j1) {
+      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(w.row + i));
+      memcpy(e, &raw, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) e[j] = w.row[min(i + j, j1 - 1)];
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const float x = sanitize(Elem<T>::to_f32(e[j]));
+      if (i + j < j1) {
+        n_ties += x == cut;
+        if (x > cut) sum += weight(x);
+      }
+    }
   }
   t_before += block_scan(s, n_ties).before;
   before += block_scan(s, sum).before;
-  const auto at = [&](u64 above, u64 t_seen) { return above + min(ties, t_seen) * wcut; };
-  if (!(at(before, t_before) <= target && target < at(before + sum, t_before + n_ties))) return;
+  if (at(before, t_before) <= target && target < at(before + sum, t_before + n_ties)) pick(j0, j1);
+}
+
+static_assert(sizeof(Queue) <= sizeof(ByValue), "the queue lies over the counts");
+
+// Rows of at most kSmall tokens: one CTA sorts (value descending, index ascending), and
+// every filter is a length of the sorted row.
+constexpr int kSmall = 2048;
+struct SmallShared {
+  Shared s;  // block_scan's
+  u64 key[kSmall];
+  u64 weight[kSmall];  // by index
+  u64 z;
+  int n;
+  uint32_t low;
+};
+
+static_assert(sizeof(SmallShared) + 1024 <= 64 * 1024, "shared memory");
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2)
+sample_small_kernel(const T* __restrict__ logits, const Params p) {
+  extern __shared__ __align__(16) uint8_t dynamic_smem[];
+  SmallShared& sm = *reinterpret_cast<SmallShared*>(dynamic_smem);
+  const int t = threadIdx.x, r = blockIdx.x, V = p.V;
+  int N = 2;
+  while (N < V) N *= 2;
+  const int per = (N + kThreads - 1) / kThreads;  // places of a thread, side by side
+  pdl_wait();
+  pdl_trigger();
+  const T* row = logits + int64_t(r) * p.row_stride;
+  const float T_ = p.temperature[r], tp = p.top_p ? p.top_p[r] : 1.f;
+  const float mp = p.min_p ? p.min_p[r] : 0.f, u = p.u[r];
+  const int k = p.top_k ? p.top_k[r] : 0;
+  for (int i = t; i < N; i += kThreads) {
+    sm.key[i] = i < V ? (u64(ord_key(sanitize(Elem<T>::to_f32(row[i])))) << 32) | ~uint32_t(i) : 0;
+    sm.weight[i] = 0;
+  }
+  if (t == 0) sm.low = 0xffffffffu;
+  __syncthreads();
 #pragma unroll 1
-  for (int i = j0; i < j1; ++i) {
-    const float x = token(i);
-    t_before += x == cut;
-    before += weight(x);
-    if (at(before, t_before) > target) {
-      write(i, x);
+  for (int size = 2; size <= N; size *= 2) {
+#pragma unroll 1
+    for (int step = size / 2; step > 0; step /= 2) {
+      for (int j = t; j < N / 2; j += kThreads) {
+        const int a = 2 * j - (j & (step - 1)), b = a + step;
+        const u64 x = sm.key[a], y = sm.key[b];
+        if ((x < y) == ((a & size) == 0)) {  // descending runs first
+          sm.key[a] = y;
+          sm.key[b] = x;
+        }
+      }
+      __syncthreads();
+    }
+  }
+  const auto value = [&](int i) { return key_value(uint32_t(sm.key[i] >> 32)); };
+  const auto index = [&](int i) { return int(~uint32_t(sm.key[i])); };
+  const float m = value(0);
+  if (!(T_ > 1e-6f) || k == 1 || tp <= 0.f || mp > 1.f) {
+    if (t == 0) {
+      p.out[r] = index(0);
+      if (p.logprobs) p.logprobs[r] = 0.f;
+    }
+    return;
+  }
+  const double T64 = double(T_), one = double(1ull << kFrac);
+  const int n_k = k > 0 && k < V ? k : V;
+  // weights in the sorted order, and how many pass min-p
+  u64 w[kSmall / kThreads] = {}, sum = 0, pass = 0;
+  uint32_t positive = 0;
+  for (int e = 0; e < per; ++e) {
+    const int i = t * per + e;
+    if (i >= n_k) break;
+    const double x = exp((double(value(i)) - double(m)) / T64);
+    w[e] = u64(__double2ll_rn(x * one));
+    sum += w[e];
+    pass += !(mp > 0.f) || x >= double(mp);
+    positive |= uint32_t(x > 0.0) << e;
+  }
+  const Scan ws = block_scan(sm.s, sum);
+  int n = max(1, int(min(block_scan(sm.s, pass).total, u64(n_k))));
+  if (tp < 1.f) {
+    const u64 target = max(u64(ceil(double(ws.total) * double(tp))), u64(1));
+    if (t == 0) sm.n = n_k;
+    __syncthreads();
+    u64 run = ws.before;
+    for (int e = 0; e < per; ++e) {
+      if (run < target && run + w[e] >= target) sm.n = t * per + e + 1;
+      run += w[e];
+    }
+    __syncthreads();
+    n = min(n, sm.n);
+  }
+  // the kept weights by index
+  for (int e = 0; e < per; ++e) {
+    const int i = t * per + e;
+    if (i >= n) break;
+    sm.weight[index(i)] = w[e];
+    if (positive >> e & 1) atomicMin(&sm.low, uint32_t(index(i)));
+  }
+  __syncthreads();
+  sum = 0;
+  for (int e = 0; e < per && t * per + e < V; ++e) sum += sm.weight[t * per + e];
+  const Scan is = block_scan(sm.s, sum);
+  const auto write = [&](int i) {
+    const float x = sanitize(Elem<T>::to_f32(row[i]));
+    p.out[r] = i;
+    if (p.logprobs)
+      p.logprobs[r] = float((double(x) - double(m)) / T64 - log(double(is.total) / one));
+  };
+  if (!(u > 0.f)) {
+    if (t == 0) write(int(sm.low));
+    return;
+  }
+  u64 target = u64(double(u) * double(is.total));
+  if (target >= is.total) target = is.total - 1;
+  if (!(is.before <= target && target < is.before + sum)) return;
+  u64 run = is.before;
+  for (int i = t * per; i < V; ++i) {
+    run += sm.weight[i];
+    if (run > target) {
+      write(i);
       return;
     }
   }
 }
-
-static_assert(sizeof(Queue) <= sizeof(ByValue), "the queue lies over the counts");
 
 // CTAs of a row's cluster: enough to fill the SMs (two CTAs each) when rows are few, at
 // least 2048 tokens each so that the exchanges do not outweigh the work, and never more
@@ -1033,6 +1338,13 @@ extern "C" int as_sample_tokens(int64_t* out, float* logprobs, const void* logit
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   auto run = [&](auto tag) -> int {
     using T = decltype(tag);
+    if (vocab <= kSmall) {  // a sort costs less than the histograms' exchanges
+      cudaFuncSetAttribute(sample_small_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           int(sizeof(SmallShared)));
+      launch_pdl(sample_small_kernel<T>, dim3(unsigned(num_rows)), dim3(kThreads),
+                 sizeof(SmallShared), s, static_cast<const T*>(logits), p);
+      return check_launch("as_sample_tokens");
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(num_rows) * p.C);
     cfg.blockDim = dim3(kThreads);

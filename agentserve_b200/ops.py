@@ -49,6 +49,26 @@ def _stream(device: torch.device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+class _on_device:
+    """`dev` as the current device for a call (nothing to do when it is), and its current
+    stream's handle as the context's value."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, dev: torch.device):
+        self.index = dev.index
+
+    def __enter__(self) -> int:
+        self.before = torch.cuda.current_device()
+        if self.index != self.before:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc) -> None:
+        if self.index != self.before:
+            torch.cuda.set_device(self.before)
+
+
 def device_status(clear: bool = True, device=None) -> int:
     """Read (and clear) the device status word: 1 bad block id, 2 bad slot, 4 wait
     timeout, 8 position outside the RoPE table, 16 sequence longer than its table row."""
@@ -313,7 +333,7 @@ class SharedPrefixPlan:
             num_seqs, num_heads, num_kv_heads, head_dim, code))
         pinned = self.device.type == "cuda"
         self._host = torch.zeros(n, dtype=torch.int32, pin_memory=pinned)
-        self._header = ctypes.c_void_p(self._host.data_ptr())
+        self._header = self._host.data_ptr()
         self.ints = torch.zeros(n, dtype=torch.int32, device=self.device)
         self._copied = torch.cuda.Event() if pinned else None
 
@@ -378,40 +398,48 @@ def shared_prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cac
     [B, >=max_blocks] int32, seq_lens_k [B] int32 (keys incl. the new token).  Returns
     out [B, H*D] in out_layout.  workspace: new_shared_prefix_workspace(plan), allocated
     and cleared per call when not given."""
-    dev = q.device
-    _cuda(q, k_cache, v_cache, block_tables, seq_lens_k, workspace, out)
+    # (the checks are written for their cost: a decode step makes this call per layer)
+    dev, dt = q.device, q.dtype
+    if not q.is_cuda:
+        raise RuntimeError("agentserve_b200 ops need CUDA tensors (no CPU fallback)")
+    _require(q.dim() == 3 and k_cache.dim() == 4, "q must be [B, H, D], k_cache [NB, 16, Kh, D]")
     B, H, D = q.shape
     NB, bs, Kh, D2 = k_cache.shape
     _require(bs == BLOCK_SIZE and D2 == D and v_cache.shape == k_cache.shape,
              "k_cache / v_cache must be [NB, 16, Kh, D] with q's head_dim")
     _require(k_cache.is_contiguous() and v_cache.is_contiguous(), "KV planes must be contiguous")
-    _require(k_cache.dtype == q.dtype and v_cache.dtype == q.dtype,
-             "k_cache / v_cache must have q's dtype")
-    _require(_row_view_ok(q) and (B == 1 or q.stride(0) >= H * D),
+    _require(k_cache.dtype is dt and v_cache.dtype is dt, "k_cache / v_cache must have q's dtype")
+    qs = q.stride()
+    _require(qs[2] == 1 and qs[1] == D and (B == 1 or qs[0] >= H * D),
              "q must be [B, H, D] with contiguous rows")
-    _require(block_tables.dtype == torch.int32 and block_tables.dim() == 2 and
-             block_tables.shape[0] == B and block_tables.shape[1] > 0 and
-             (block_tables.stride(1) == 1 or block_tables.shape[1] == 1),
+    _require(block_tables.dtype is torch.int32 and block_tables.dim() == 2, "block_tables must be "
+             "int32 [B, max_blocks] with contiguous rows")
+    tb, mb = block_tables.shape
+    ts = block_tables.stride()
+    _require(tb == B and mb > 0 and (ts[1] == 1 or mb == 1),
              "block_tables must be int32 [B, max_blocks] with contiguous rows")
-    _require(seq_lens_k.dtype == torch.int32 and seq_lens_k.shape == (B,) and
-             seq_lens_k.is_contiguous(), "seq_lens_k must be a contiguous int32 [B]")
-    _require(plan.dtype == q.dtype and plan.num_seqs == B, "the plan was made for another batch")
-    for t in (k_cache, v_cache, block_tables, seq_lens_k, plan.ints, workspace, out):
-        _require(t is None or t.device == dev, "all tensors must be on q's device")
+    _require(seq_lens_k.dtype is torch.int32 and seq_lens_k.shape == (B,) and
+             (B == 1 or seq_lens_k.stride(0) == 1), "seq_lens_k must be a contiguous int32 [B]")
+    _require(plan.dtype is dt and plan.num_seqs == B, "the plan was made for another batch")
     if out is None:
-        out = torch.empty(B, H * D, dtype=q.dtype, device=dev)
-    _require(out.shape == (B, H * D) and out.dtype == q.dtype and out.is_contiguous(),
-             "out must be a contiguous [B, H*D] of q's dtype")
+        out = torch.empty(B, H * D, dtype=dt, device=dev)
+    else:
+        _require(out.shape == (B, H * D) and out.dtype is dt and out.is_contiguous(),
+                 "out must be a contiguous [B, H*D] of q's dtype")
     if workspace is None:
         workspace = new_shared_prefix_workspace(plan)
-    bt_stride = block_tables.stride(0) if B > 1 else block_tables.shape[1]
-    with torch.cuda.device(dev):
-        N.check(N.load().as_shared_prefix_decode_attention(
-            _ptr(out), _ptr(q), q.stride(0) if B > 1 else H * D, _ptr(k_cache), _ptr(v_cache),
-            _ptr(block_tables), bt_stride, _ptr(seq_lens_k), plan._header, _ptr(plan.ints), B, H,
-            Kh, D, BLOCK_SIZE, NB, block_tables.shape[1], float(scale), _ptr(workspace),
-            workspace.numel() * workspace.element_size(), int(out_layout), dtype_code(q.dtype),
-            _stream(dev)), "as_shared_prefix_decode_attention")
+    _require(workspace.is_contiguous(), "workspace must be contiguous")
+    for t in (k_cache, v_cache, block_tables, seq_lens_k, plan.ints, workspace, out):
+        if t.device != dev:
+            raise ValueError("all tensors must be on q's device")
+    with _on_device(dev) as stream:
+        rc = N.load().as_shared_prefix_decode_attention(
+            out.data_ptr(), q.data_ptr(), qs[0] if B > 1 else H * D, k_cache.data_ptr(),
+            v_cache.data_ptr(), block_tables.data_ptr(), ts[0] if B > 1 else mb,
+            seq_lens_k.data_ptr(), plan._header, plan.ints.data_ptr(), B, H, Kh, D, BLOCK_SIZE, NB,
+            mb, scale, workspace.data_ptr(), workspace.nbytes, out_layout, _DTYPES[dt], stream)
+    if rc:
+        N.check(rc, "as_shared_prefix_decode_attention")
     return out
 
 
@@ -554,25 +582,33 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tens
     at which the running sum of probabilities exceeds u.  u, temperature, top_p and
     min_p are fp32 [B], top_k int32 [B]; logprobs (fp32 [B], optional) receives the log
     of the token's probability among the kept ones.  See as_sample_tokens."""
-    _cuda(logits, u, temperature, top_k, top_p, min_p, out, logprobs)
-    _require(logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1),
-             "sample_tokens: logits must be [B, V] with contiguous rows")
+    dev = logits.device
+    if not logits.is_cuda:
+        raise RuntimeError("agentserve_b200 ops need CUDA tensors (no CPU fallback)")
+    _require(logits.dim() == 2, "sample_tokens: logits must be [B, V] with contiguous rows")
     B, V = logits.shape
+    ls = logits.stride()
+    _require(ls[1] == 1 or V == 1, "sample_tokens: logits must be [B, V] with contiguous rows")
+    code = dtype_code(logits.dtype)
+    if out is None:
+        out = torch.empty(B, dtype=torch.int64, device=dev)
     for name, t, dt in (("u", u, torch.float32), ("temperature", temperature, torch.float32),
                         ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
                         ("min_p", min_p, torch.float32), ("logprobs", logprobs, torch.float32),
                         ("out", out, torch.int64)):
-        if t is not None and not (t.dtype == dt and t.shape == (B,) and t.is_contiguous()
-                                  and t.device == logits.device):
+        if t is not None and not (t.dtype is dt and t.shape == (B,) and
+                                  (B <= 1 or t.stride(0) == 1) and t.device == dev):
             raise ValueError(f"sample_tokens: {name} must be a contiguous {dt} [B] on the "
                              "logits' device")
-    if out is None:
-        out = torch.empty(B, dtype=torch.int64, device=logits.device)
-    with torch.cuda.device(logits.device):
-        N.check(N.load().as_sample_tokens(
-            _ptr(out), _ptr(logprobs), _ptr(logits), logits.stride(0) if B > 1 else V, _ptr(u),
-            _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), B, V,
-            dtype_code(logits.dtype), _stream(logits.device)), "as_sample_tokens")
+    with _on_device(dev) as stream:
+        rc = N.load().as_sample_tokens(
+            out.data_ptr(), None if logprobs is None else logprobs.data_ptr(), logits.data_ptr(),
+            ls[0] if B > 1 else V, u.data_ptr(), temperature.data_ptr(),
+            None if top_k is None else top_k.data_ptr(),
+            None if top_p is None else top_p.data_ptr(),
+            None if min_p is None else min_p.data_ptr(), B, V, code, stream)
+    if rc:
+        N.check(rc, "as_sample_tokens")
     return out
 
 

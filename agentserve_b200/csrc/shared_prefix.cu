@@ -480,7 +480,7 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
     int64_t own_most = kMinOwn;
     for (int b = 0; b < B; ++b) own_most = std::max<int64_t>(own_most, row_blocks[b] - shared[b]);
     const int64_t own_piece =
-        best_piece(n.tc ? kMinOwn : 2, own_most, n.own_slots, 4, n.tc ? kOwnOverhead : 4,
+        best_piece(kMinOwn, own_most, n.own_slots, 4, n.tc ? kOwnOverhead : 8,
                    [&](int64_t piece) {
           int64_t items = 0;
           for (int b = 0; b < B; ++b) items += own_splits(b, piece);

@@ -17,6 +17,7 @@ from .policies import (FifoPolicy, PriorityPolicy, SchedulerPolicy,  # noqa: F40
                        TrajectoryDeadlinePolicy, TrajectoryProgressPolicy)
 from .prefix_cache import PrefixCache  # noqa: F401
 from .request import Request, RequestStatus  # noqa: F401
+from .sampling import SamplingParams, UniformStream  # noqa: F401
 from .scheduler import Scheduler  # noqa: F401
 
 __version__ = "0.2.0"

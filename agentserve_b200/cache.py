@@ -17,8 +17,9 @@ changes is where the data lives:
 from __future__ import annotations
 
 from collections import deque
-from typing import Dict, List, Optional, Sequence
+from typing import Dict, List, Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
 from . import ops
@@ -43,6 +44,10 @@ class DeviceBlockAllocator:
         self._free: deque[int] = deque(range(num_blocks))
         self._used: set[int] = set()
         self._request_blocks: Dict[str, List[int]] = {}
+        # counts the changes of any request's block list (shared_prefix_groups' answers
+        # hold until the next one)
+        self.epoch = 0
+        self._block_arrays: Dict[str, np.ndarray] = {}
         # device block-table rows
         self.max_seqs = max_seqs
         self.max_blocks_per_seq = max_blocks_per_seq or num_blocks
@@ -89,6 +94,7 @@ class DeviceBlockAllocator:
             self._used.add(b)
             out.append(b)
         self._request_blocks.setdefault(request_id, []).extend(out)
+        self._changed(request_id)
         if out:
             self.block_tables[row, have:have + len(out)].copy_(self._host_ints(out, torch.int32),
                                                                non_blocking=True)
@@ -100,6 +106,7 @@ class DeviceBlockAllocator:
 
     def free(self, request_id: str) -> None:
         """cache.py:103-111, plus releasing the device table row."""
+        self._changed(request_id)
         for b in self._request_blocks.pop(request_id, []):
             self._ref[b] -= 1
             if self._ref[b] == 0:
@@ -155,9 +162,91 @@ class DeviceBlockAllocator:
         for b in ids:
             self._ref[b] += 1
         self._request_blocks[request_id] = list(ids)
+        self._changed(request_id)
         if ids:
             self.block_tables[row, :len(ids)].copy_(self._host_ints(ids, torch.int32),
                                                     non_blocking=True)
+
+    def _changed(self, request_id: str) -> None:
+        self.epoch += 1
+        self._block_arrays.pop(request_id, None)
+
+    def shared_prefix_groups(self, request_ids: Sequence[str], min_saved: int = 1
+                             ) -> Tuple[List[List[int]], List[int]]:
+        """Groups of a decode batch for ops.shared_prefix_plan: (groups, prefix_blocks),
+        lists of positions in request_ids whose block lists begin with the same blocks, and
+        how many.  A request is in at most one group; of all groupings along shared
+        beginnings (a system prompt, the longer histories of sessions below it) one that
+        saves most block reads is taken.  Groups that save fewer than min_saved block
+        reads are left out."""
+        arrays = []
+        for r in request_ids:
+            a = self._block_arrays.get(r)
+            if a is None:
+                a = self._block_arrays[r] = np.array(self._request_blocks.get(r, ()),
+                                                     dtype=np.int64)
+            arrays.append(a)
+
+        def node(rows: List[int], depth: int, level: int = 0):
+            """(blocks all rows agree on, rows ending there, nodes and single rows below)."""
+            least = min(len(arrays[r]) for r in rows)
+            first = arrays[rows[0]]
+            while depth < least:  # a stretch at a time: most rows agree on long ones
+                end = min(least, depth + 256)
+                same = (np.stack([arrays[r][depth:end] for r in rows]) == first[depth:end]).all(0)
+                n = end - depth if same.all() else int(same.argmin())
+                depth += n
+                if n < same.size:
+                    break
+            if level == 64:  # a chain of histories deeper than that is not divided further
+                return depth, list(rows), []
+            below: Dict[int, List[int]] = {}
+            for r in rows:
+                if len(arrays[r]) > depth:
+                    below.setdefault(int(arrays[r][depth]), []).append(r)
+            alone = [r for r in rows if len(arrays[r]) == depth]
+            alone += [x[0] for x in below.values() if len(x) == 1]
+            return depth, alone, [node(x, depth, level + 1) for x in below.values() if len(x) > 1]
+
+        def best(tree, above: int):
+            """(saved reads, groups, rows left to the group open above) below a node, when a
+            group on `above` blocks is open above it (0: none): a row in a group on n
+            blocks saves n, and every group reads its own blocks once."""
+            depth, alone, below = tree
+            known = memo.get((id(tree), above))
+            if known is not None:
+                return known
+
+            def with_open(n):
+                saved, groups, left = len(alone) * n, [], list(alone)
+                for t in below:
+                    v, g, rest = best(t, n)
+                    saved += v
+                    groups += g
+                    left += rest
+                return saved, groups, left
+
+            answer = with_open(above)
+            if depth > above:
+                v, g, rest = with_open(depth)
+                if v - depth > answer[0]:
+                    answer = v - depth, g + [(rest, depth)], []
+            memo[id(tree), above] = answer
+            return answer
+
+        starts: Dict[int, List[int]] = {}
+        for i, a in enumerate(arrays):
+            if len(a):
+                starts.setdefault(int(a[0]), []).append(i)
+        groups, blocks = [], []
+        for rows in starts.values():
+            if len(rows) > 1:
+                tree, memo = node(rows, 0), {}
+                for g, n in best(tree, 0)[1]:
+                    if (len(g) - 1) * n >= max(1, min_saved):
+                        groups.append(sorted(g))
+                        blocks.append(n)
+        return groups, blocks
 
     def ref_count(self, block_id: int) -> int:
         return self._ref[block_id]

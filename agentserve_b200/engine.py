@@ -26,8 +26,10 @@ underneath is the device path:
   reference admits it without blocks (engine.py:286-289), which only its CPU mock
   model survives.
 
-Sampling is greedy (temperature 0, sampling.py:46-58); other temperatures are
-rejected.  The difficulty classifier and output-length predictor of AgentServe are
+Sampling is greedy at temperature 0 (sampling.py:46-58); at other temperatures the
+batch's tokens are drawn in one launch with temperature, top-k, top-p and min-p, from
+numbers that depend on the seed, the request and the token's index alone (a model
+without sampled steps rejects them).  The difficulty classifier and output-length predictor of AgentServe are
 optional collaborators: pass objects with `classify(prompt)` (returning .level.value,
 .priority, .estimated_output_tokens) and `predict(prompt)` / `update(prompt, n)`;
 without them the request's own difficulty, priority and estimate are used.
@@ -45,6 +47,7 @@ import torch
 from .cache import DeviceBlockAllocator
 from .model import B200LlamaModel
 from .prefix_cache import PrefixCache
+from .sampling import SamplingParams, UniformStream
 from .scheduler import Scheduler
 
 
@@ -107,15 +110,27 @@ class B200Engine:
                  scheduler_policy=None, use_relative_batching: bool = False,
                  use_combined_batching: bool = False, classifier=None, predictor=None,
                  scheduler=None, max_seqs: int = 1024,
-                 max_blocks_per_seq: Optional[int] = None):
-        if temperature > 1e-6:
-            raise ValueError("B200Engine samples greedily (temperature 0); "
+                 max_blocks_per_seq: Optional[int] = None, min_p: float = 0.0, seed: int = 0,
+                 per_request_sampling: bool = False, shared_prefix_attention: bool = False):
+        """per_request_sampling: every request's own temperature, top_p, top_k and min_p
+        instead of the engine's.  shared_prefix_attention: decode steps read the blocks
+        that requests share (prefix-cache hits) once per group of them."""
+        self.sampling = SamplingParams(temperature, top_k, top_p, min_p)
+        self.per_request_sampling = per_request_sampling
+        self._uniform = UniformStream(seed)
+        self._samples = per_request_sampling or not self.sampling.greedy
+        if self._samples and model is not None and not hasattr(model, "prefill_paged_sampled"):
+            raise ValueError("the model has greedy steps only (temperature 0); "
                              f"temperature={temperature} is not supported")
         self.config = config
         self.eos_token_id = eos_token_id
         self.temperature, self.top_p, self.top_k = temperature, top_p, top_k
         self.model = model if model is not None else B200LlamaModel(config, dtype=dtype,
                                                                     device=device)
+        if shared_prefix_attention:
+            if not hasattr(self.model, "shared_prefix_decode"):
+                raise ValueError("the model has no shared-prefix decode attention")
+            self.model.shared_prefix_decode = True
         self.device = self.model.device
         dtype = self.model.dtype
         # decode batches come in many (batch size, block bucket) shapes: keep their
@@ -207,6 +222,18 @@ class B200Engine:
         self.allocator.free(req.request_id)
         self._frozen.pop(req.request_id, None)
         self._hashes.pop(req.request_id, None)
+        self._uniform.forget(req.request_id)
+
+    # ------------------------------------------------------------------ sampling
+    def _draws(self, batch: List, ahead: int = 0) -> tuple:
+        """(settings, numbers) for each request's next token, or the one `ahead` after."""
+        if self.per_request_sampling:
+            params = [SamplingParams(r.temperature, r.top_k, r.top_p, getattr(r, "min_p", 0.0))
+                      for r in batch]
+        else:
+            params = [self.sampling] * len(batch)
+        return params, self._uniform([r.request_id for r in batch],
+                                     [r.num_output_tokens + ahead for r in batch])
 
     def _prompt_hashes(self, req) -> List[int]:
         """The prompt's chained block hashes, computed once per request (admission
@@ -281,9 +308,12 @@ class B200Engine:
             frozen = self._frozen.get(req.request_id, 0)
             if req.num_cached_tokens < frozen:
                 req.num_cached_tokens = frozen
-        first = self.model.prefill_paged_greedy([r.token_ids for r in batch],
-                                                [r.num_cached_tokens for r in batch],
-                                                self.allocator, [r.request_id for r in batch])
+        args = ([r.token_ids for r in batch], [r.num_cached_tokens for r in batch],
+                self.allocator, [r.request_id for r in batch])
+        if self._samples:
+            first = self.model.prefill_paged_sampled(*args, *self._draws(batch))
+        else:
+            first = self.model.prefill_paged_greedy(*args)
         for req, tok in zip(batch, first):
             req.num_cached_tokens = len(req.token_ids)
             self.scheduler.on_prefill_complete(req)
@@ -315,7 +345,13 @@ class B200Engine:
         spec, self._spec = self._spec, None
         rids = [r.request_id for r in batch]
         seq_lens = [r.num_cached_tokens + r.num_output_tokens - 1 for r in batch]
-        launch = getattr(self.model, "decode_paged_greedy_launch", None)
+        if self._samples:
+            def launch(last, lens, allocator, ids, feed_from=None):
+                return self.model.decode_paged_sampled_launch(
+                    last, lens, allocator, ids, *self._draws(batch, feed_from is not None),
+                    feed_from=feed_from)
+        else:
+            launch = getattr(self.model, "decode_paged_greedy_launch", None)
         pick = spec.positions_of(batch) if spec is not None else None
         if pick is not None:
             handle, take = spec.handle, pick

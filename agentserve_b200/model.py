@@ -29,12 +29,14 @@ import math
 from collections import OrderedDict
 from typing import List, Optional, Sequence
 
+import numpy as np
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _native as N
 from . import ops
+from . import sampling as S
 from .cache import DeviceBlockAllocator
 
 BS = ops.BLOCK_SIZE
@@ -187,6 +189,18 @@ class B200LlamaModel(nn.Module):
         # attention launch (as_rope_paged_decode_attention, bf16/fp16, head_dim 64/128);
         # False: separate RoPE + cache-write launch first (same results, bit for bit)
         self.fused_rope_decode: bool = True
+        # True: a paged decode step whose requests share leading blocks (prefix-cache hits)
+        # reads and multiplies those once per group (ops.shared_prefix_decode_attention).
+        # Off by default: the results differ from the per-request attention's in rounding.
+        self.shared_prefix_decode: bool = False
+        # Block reads (members - 1 times shared blocks, over all groups) that sharing must
+        # save: below, the per-request launch is faster.  B200, rotation included, per
+        # layer, fused against shared: 16 sequences on 64 blocks (960 saved) 12.8 / 17.4 us
+        # at head_dim 64 and 19.0 / 20.9 at 128; on 128 (1,920) 18.4 / 18.1 and 31.8 /
+        # 22.3; 64 on 32 (2,016) 22.9 / 23.3 and 40.7 / 29.6; 64 on 256 61.0 / 29.2 and
+        # 112 / 38.8.
+        self.shared_prefix_min_saved: int = 1920
+        self._prefix_groups: Optional[tuple] = None  # (allocator, its epoch, requests, groups)
         self.max_decode_graphs: int = 16
         self._graphs: "OrderedDict[tuple, _PagedStepGraph]" = OrderedDict()
         self._graph_pool = None
@@ -384,6 +398,20 @@ class B200LlamaModel(nn.Module):
         return greedy(self.forward_prefill_paged(token_ids, num_cached, allocator,
                                                  request_ids)).tolist()
 
+    @torch.inference_mode()
+    def prefill_paged_sampled(self, token_ids: Sequence[Sequence[int]],
+                              num_cached: Sequence[int], allocator, request_ids: Sequence[str],
+                              sampling: Sequence["S.SamplingParams"],
+                              u: Sequence[float]) -> List[int]:
+        """prefill_paged_greedy with each request's own sampling settings and its uniform
+        number (engine.py:321)."""
+        if len(sampling) != len(token_ids) or len(u) != len(token_ids):
+            raise ValueError("prefill_paged_sampled needs one setting and one number per request")
+        if len(token_ids) == 0:
+            return []
+        return sample(self.forward_prefill_paged(token_ids, num_cached, allocator, request_ids),
+                      sampling, u).tolist()
+
     # ------------------------------------------------------------------ decode (lists)
     @torch.inference_mode()
     def forward_decode_batch(self, last_token_ids: List[int], kv_caches: list,
@@ -551,20 +579,27 @@ class B200LlamaModel(nn.Module):
     def _decode_core(self, tokens: torch.Tensor, seq_lens: torch.Tensor, row_ids: torch.Tensor,
                      allocator: DeviceBlockAllocator, max_blocks: int, bps: int,
                      positions: Optional[torch.Tensor] = None,
-                     ws: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     ws: Optional[torch.Tensor] = None,
+                     shared: Optional[tuple] = None) -> torch.Tensor:
         """One decode step entirely on the device (no host sync): pack -> per layer
         (norm, fused QKV GEMM, fused RoPE+cache write, paged attention, o_proj,
         MLP) -> norm -> lm_head.  Returns logits [B, V].  A CUDA graph passes its own
-        split-K workspace `ws` (the shared one may be reallocated by later calls)."""
+        split-K workspace `ws` (the shared one may be reallocated by later calls).
+        shared: (plan, workspace) of a batch whose requests share leading blocks."""
         B = tokens.shape[0]
         pk = ops.pack_decode(allocator.block_tables, seq_lens, row_ids, max_blocks)
         pos = pk.positions if positions is None else positions
-        if ws is None:
+        if ws is None and shared is None:
             ws = self._workspace(B, max_blocks, bps)
 
         def attention(li, layer, h):
             q, k, v = self._qkv(layer, h)
             kp, vp = allocator.k_plane(li), allocator.v_plane(li)
+            if shared is not None:
+                ops.rope_reshape_and_cache(q, k, v, pos, pk.slot_mapping, self.rope_table, kp, vp)
+                return ops.shared_prefix_decode_attention(
+                    q, kp, vp, pk.block_tables, pk.seq_lens_k, shared[0], self.scale, shared[1],
+                    out_layout=self.decode_layout)
             if self.fused_rope_decode and ops.rope_decode_fusable(q, kp):
                 return ops.rope_paged_decode_attention(
                     q, k, v, pos, pk.slot_mapping, self.rope_table, kp, vp, pk.block_tables,
@@ -595,7 +630,7 @@ class B200LlamaModel(nn.Module):
         if (self.decode_graphs and dev.type == "cuda" and
                 (position_offsets is seq_lens or list(position_offsets) == list(seq_lens))):
             return self._graphed_decode(allocator, last_token_ids, seq_lens, rows, max_blocks,
-                                        bps), None
+                                        bps, self._sharing(allocator, request_ids)), None
         host = torch.tensor([list(last_token_ids), list(seq_lens), rows, list(position_offsets)],
                             dtype=torch.int64).pin_memory()
         d = host.to(dev, non_blocking=True)
@@ -603,34 +638,64 @@ class B200LlamaModel(nn.Module):
         sl = d[1].to(torch.int32)
         rid = d[2].to(torch.int32)
         pos = None if list(position_offsets) == list(seq_lens) else d[3].contiguous()
-        logits = self._decode_core(tokens, sl, rid, allocator, max_blocks, bps, positions=pos)
+        logits = self._decode_core(tokens, sl, rid, allocator, max_blocks, bps, positions=pos,
+                                   shared=self._shared_plan(allocator, request_ids, B))
         return logits, None
 
+    def _sharing(self, allocator, request_ids: Sequence[str], batch: int = 0) -> Optional[tuple]:
+        """(groups, prefix_blocks, row_blocks) of the batch where its requests share enough
+        leading blocks, else None.  batch > len(request_ids): padding rows of one block."""
+        if not self.shared_prefix_decode or len(request_ids) < 2:
+            return None
+        known = self._prefix_groups
+        rids = tuple(request_ids)
+        if not (known is not None and known[0] is allocator and known[1] == allocator.epoch
+                and known[2] == rids):
+            groups, blocks = allocator.shared_prefix_groups(rids)
+            if sum((len(g) - 1) * n for g, n in zip(groups, blocks)) < self.shared_prefix_min_saved:
+                groups, blocks = [], []
+            known = self._prefix_groups = (allocator, allocator.epoch, rids, groups, blocks)
+        if not known[3]:
+            return None
+        rows = [len(allocator._request_blocks[r]) for r in rids]
+        return known[3], known[4], rows + [1] * (batch - len(rows))
+
+    def _shared_plan(self, allocator, request_ids: Sequence[str], batch: int) -> Optional[tuple]:
+        """(plan, workspace) for one eager step, or None."""
+        sharing = self._sharing(allocator, request_ids, batch)
+        if sharing is None:
+            return None
+        plan = ops.shared_prefix_plan(*sharing, self.H, self.Kh, self.D, self.dtype, self.device)
+        return plan, ops.new_shared_prefix_workspace(plan)
 
     def _graphed_decode(self, allocator, tokens, seq_lens, rows, max_blocks: int,
-                        bps: int, sample: bool = False) -> torch.Tensor:
+                        bps: int, sharing: Optional[tuple] = None) -> torch.Tensor:
         """forward_decode_paged through a cached CUDA graph.  Graphs are keyed by the
         allocator, the batch size and max_blocks rounded up to a power of two (capped by
         the allocator's table width); the split-K decomposition follows that bucket.
-        sample=True captures greedy sampling too and returns next tokens instead of
-        logits.  Least recently used graphs beyond max_decode_graphs are released."""
-        g = self._step_graph(allocator, len(tokens), max_blocks, bps, sample)
+        sharing: the batch's groups (_sharing), for the graphs with that attention.
+        Least recently used graphs beyond max_decode_graphs are released."""
+        g = self._step_graph(allocator, len(tokens), max_blocks, bps, "", sharing)
         return g.run(tokens, seq_lens, rows)
 
-    def _step_graph(self, allocator, B: int, max_blocks: int, bps: int,
-                    sample: bool) -> "_PagedStepGraph":
+    def _step_graph(self, allocator, B: int, max_blocks: int, bps: int, sample: str,
+                    sharing: Optional[tuple] = None) -> "_PagedStepGraph":
+        """sample: "" (the graph gives logits), "greedy" or "sampled" (next tokens)."""
         cap = allocator.block_tables.shape[1]
         mb = min(cap, 1 << max(0, (max_blocks - 1).bit_length()))
-        key = (id(allocator), B, mb, bps, sample)
+        key = (id(allocator), B, mb, bps, sample, sharing is not None)
         g = self._graphs.get(key)
         if g is None or g.allocator is not allocator:
             if self._graph_pool is None:
                 self._graph_pool = torch.cuda.graph_pool_handle()
-            g = _PagedStepGraph(self, allocator, B, mb, bps, self._graph_pool, sample)
+            g = _PagedStepGraph(self, allocator, B, mb, bps, self._graph_pool, sample,
+                                sharing is not None)
             self._graphs[key] = g
             while len(self._graphs) > self.max_decode_graphs:
                 self._graphs.popitem(last=False)
         self._graphs.move_to_end(key)
+        if sharing is not None:
+            g.set_sharing(sharing)
         return g
 
     @torch.inference_mode()
@@ -656,8 +721,34 @@ class B200LlamaModel(nn.Module):
         batch, in the same order) the input tokens are that step's outputs, read on the
         device, so this step can be queued before the previous one's tokens reach the
         host; last_token_ids is then ignored."""
+        return self._decode_launch(last_token_ids, seq_lens, allocator, request_ids, None, None,
+                                   feed_from)
+
+    @torch.inference_mode()
+    def decode_paged_sampled(self, last_token_ids: List[int], seq_lens: List[int], allocator,
+                             request_ids: List[str], sampling: Sequence["S.SamplingParams"],
+                             u: Sequence[float]) -> List[int]:
+        """decode_paged_greedy with each request's own sampling settings and its uniform
+        number u in [0, 1) (sampling.py's sampled branch, engine.py:379-383), in the same
+        graph and with the same one copy of all tokens."""
+        return self.decode_paged_sampled_launch(last_token_ids, seq_lens, allocator, request_ids,
+                                                sampling, u).result()
+
+    @torch.inference_mode()
+    def decode_paged_sampled_launch(self, last_token_ids: Optional[List[int]],
+                                    seq_lens: List[int], allocator, request_ids: List[str],
+                                    sampling: Sequence["S.SamplingParams"], u: Sequence[float],
+                                    feed_from: Optional["DecodeHandle"] = None) -> "DecodeHandle":
+        """decode_paged_sampled without waiting, as decode_paged_greedy_launch."""
+        if len(sampling) != len(seq_lens) or len(u) != len(seq_lens):
+            raise ValueError("decode_paged_sampled needs one setting and one number per request")
+        return self._decode_launch(last_token_ids, seq_lens, allocator, request_ids, sampling, u,
+                                   feed_from)
+
+    def _decode_launch(self, last_token_ids, seq_lens, allocator, request_ids, sampling, u,
+                       feed_from) -> "DecodeHandle":
         if not isinstance(allocator, DeviceBlockAllocator):
-            raise TypeError("decode_paged_greedy needs an agentserve_b200.DeviceBlockAllocator")
+            raise TypeError("paged decode needs an agentserve_b200.DeviceBlockAllocator")
         self.fuse_projections_()
         B = len(seq_lens)
         if B == 0:
@@ -677,12 +768,15 @@ class B200LlamaModel(nn.Module):
             d = host.to(self.device)
             tok = d[0] if feed_from is None else feed_from.tokens.to(torch.int64)
             logits = self._decode_core(tok, d[1].to(torch.int32), d[2].to(torch.int32),
-                                       allocator, max_blocks, self.decode_blocks_per_split)
-            out = greedy(logits)
+                                       allocator, max_blocks, self.decode_blocks_per_split,
+                                       shared=self._shared_plan(allocator, request_ids, Bp))
+            out = greedy(logits) if sampling is None else sample(logits, sampling, u)
             return DecodeHandle(out, None, B, out[:B].tolist())
-        g = self._step_graph(allocator, Bp, max_blocks, self.decode_blocks_per_split, True)
+        g = self._step_graph(allocator, Bp, max_blocks, self.decode_blocks_per_split,
+                             "greedy" if sampling is None else "sampled",
+                             self._sharing(allocator, request_ids, Bp))
         return g.launch(last_token_ids, seq_lens, rows, B,
-                        None if feed_from is None else feed_from.tokens)
+                        None if feed_from is None else feed_from.tokens, sampling, u)
 
     def release_decode_graphs(self) -> None:
         """Drop every cached decode graph now (e.g. before destroying a process group
@@ -708,20 +802,28 @@ def _batch_bucket(B: int) -> int:
 
 
 class _PagedStepGraph:
-    """One captured forward_decode_paged step (logits only) for a fixed batch size and
-    block bucket.  Inputs travel in one pinned int32 [3, B] buffer (tokens, seq_lens,
-    table rows) with one host-to-device copy per call."""
+    """One captured forward_decode_paged step for a fixed batch size and block bucket,
+    giving logits or, with greedy or sampled tokens, those.  Inputs travel in one pinned
+    int32 [3, B] buffer (tokens, seq_lens, table rows; [8, B] with the sampling settings
+    and numbers) with one host-to-device copy per call.  With `sharing`, the attention's
+    plan lives in buffers of the graph's own and is replaced when the groups change."""
 
     def __init__(self, model: "B200LlamaModel", allocator: DeviceBlockAllocator, B: int,
-                 max_blocks: int, bps: int, pool, sample: bool = False):
+                 max_blocks: int, bps: int, pool, sample: str = "", sharing: bool = False):
         self.allocator = allocator
         self.sample = sample
         dev = model.device
-        self.host = torch.zeros(3, B, dtype=torch.int32).pin_memory()
+        n = 3 + (S.STAGED if sample == "sampled" else 0)
+        self.host = torch.zeros(n, B, dtype=torch.int32).pin_memory()
         self._host_np = self.host.numpy()
-        self.inputs = torch.zeros(3, B, dtype=torch.int32, device=dev)
+        self.inputs = torch.zeros(n, B, dtype=torch.int32, device=dev)
         self.copied = torch.cuda.Event()
-        self.ws = ops.new_decode_workspace(B, model.H, model.Kh, model.D, max_blocks, bps, dev)
+        self.ws = self.shared = self._groups = None
+        if sharing:
+            plan = ops.SharedPrefixPlan(B, model.H, model.Kh, model.D, model.dtype, dev, True)
+            self.shared = (plan, ops.new_shared_prefix_workspace(plan))
+        else:
+            self.ws = ops.new_decode_workspace(B, model.H, model.Kh, model.D, max_blocks, bps, dev)
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.model, self.max_blocks, self.bps = model, max_blocks, bps
         self._pool = pool
@@ -731,9 +833,19 @@ class _PagedStepGraph:
             self.out_ready = [torch.cuda.Event(), torch.cuda.Event()]
             self._flip = 0
 
+    def set_sharing(self, sharing: tuple) -> None:
+        """The batch's groups, shared blocks and blocks per row for the next replay."""
+        if sharing != self._groups:
+            self.shared[0].load(*sharing)
+            self._groups = sharing
+
     def _body(self) -> torch.Tensor:
         logits = self.model._decode_core(self.inputs[0], self.inputs[1], self.inputs[2],
-                                         self.allocator, self.max_blocks, self.bps, ws=self.ws)
+                                         self.allocator, self.max_blocks, self.bps, ws=self.ws,
+                                         shared=self.shared)
+        if self.sample == "sampled":
+            f = self.inputs.view(torch.float32)
+            return ops.sample_tokens(logits, f[7], f[3], self.inputs[4], f[5], f[6])
         return greedy(logits) if self.sample else logits
 
     def release(self) -> None:
@@ -742,10 +854,12 @@ class _PagedStepGraph:
             self.graph = None
         self.logits = None
 
-    def _stage(self, tokens, seq_lens, rows) -> None:
+    def _stage(self, tokens, seq_lens, rows, sampling=None, u=None) -> None:
         self.copied.synchronize()  # the previous call's copy has left the pinned buffer
         h = self._host_np
         h[0], h[1], h[2] = tokens, seq_lens, rows
+        if sampling is not None:
+            S.stage(h[3:], sampling, u)
         self.inputs.copy_(self.host, non_blocking=True)
         self.copied.record()
 
@@ -755,11 +869,11 @@ class _PagedStepGraph:
         self._replay()
         return self.logits.clone()
 
-    def launch(self, tokens, seq_lens, rows, n: int,
-               feed: Optional[torch.Tensor] = None) -> "DecodeHandle":
-        """Queue one greedy step (sample=True graphs); feed: device tokens to use instead
+    def launch(self, tokens, seq_lens, rows, n: int, feed: Optional[torch.Tensor] = None,
+               sampling=None, u=None) -> "DecodeHandle":
+        """Queue one step of a graph that gives tokens; feed: device tokens to use instead
         of `tokens` (the previous step's output of the same batch)."""
-        self._stage(tokens, seq_lens, rows)
+        self._stage(tokens, seq_lens, rows, sampling, u)
         if feed is not None:
             self.inputs[0].copy_(feed)
         self._replay()
@@ -810,6 +924,17 @@ def greedy(logits: torch.Tensor) -> torch.Tensor:
     """sampling.py:46-58 with temperature <= 1e-6 (fp32, nan_to_num(0, 1e4, -1e4),
     first argmax) for [B, V] logits, in one kernel (as_greedy_argmax)."""
     return ops.greedy_argmax(logits)
+
+
+def sample(logits: torch.Tensor, sampling: Sequence["S.SamplingParams"],
+           u: Sequence[float]) -> torch.Tensor:
+    """Tokens [B] of [B, V] logits under one SamplingParams and one uniform number per
+    row (sampling.py's sampled branch), in one kernel; rows past the settings are greedy."""
+    host = torch.zeros(S.STAGED, logits.shape[0], dtype=torch.int32)
+    S.stage(host.numpy(), sampling, u)
+    d = host.pin_memory().to(logits.device, non_blocking=True)
+    f = d.view(torch.float32)
+    return ops.sample_tokens(logits, f[4], f[0], d[1], f[2], f[3])
 
 
 class DecodeGraph:

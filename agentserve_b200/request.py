@@ -59,6 +59,8 @@ class Request:
     total_steps: int = 1
     deadline: float = float("inf")
 
+    min_p: float = 0.0  # with per-request sampling; not in AgentServe's Request
+
     @property
     def num_prompt_tokens(self) -> int:
         return len(self.token_ids)

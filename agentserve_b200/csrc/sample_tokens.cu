@@ -15,8 +15,8 @@
 // over the values' bits, until one value is left.
 //
 // Sums decide between neighbouring tokens, and a border token can weigh 1e-6 of the
-// total: weights are computed in 64 bits and summed in fixed point (2^-45 at 128K
-// tokens), which makes every sum exact and independent of the order of the atomics.
+// total: weights are computed in 64 bits and summed in fixed point (units of 2^-42 of
+// the largest), which makes every sum exact and independent of the order of the atomics.
 //
 // A row is worked on by a cluster of 1 to 8 CTAs, each holding a run of indexes, its warps
 // runs of that; they exchange totals over distributed shared memory.  Every decision
@@ -40,12 +40,14 @@ constexpr int kBins = 1 << kBinBits;
 constexpr float kWindow = 12.f;  // nats covered by the first histogram
 constexpr int kTable = 512;      // 2^(i / 512)
 constexpr int kMaxVocab = 1 << 20;
-constexpr int kMaxRun = 1 << 17;  // tokens of a CTA
-// A weight is at most 1 = 2^43 units: the sum of kMaxVocab of them fits 64 bits, and its
-// three pieces of 15 bits, summed over a CTA's tokens, fit 32 bits each.
-constexpr int kFrac = 43;
-constexpr int kPiece = 15;
+constexpr int kMaxRun = (1 << 17) + 256;  // tokens of a CTA
+// A weight is at most 1 = 2^42 units: the sum of kMaxVocab of them fits 64 bits, and its
+// three pieces of 14 bits, summed over a CTA's tokens, fit 32 bits each.
+constexpr int kFrac = 42;
+constexpr int kPiece = 14;
 typedef unsigned long long u64;
+static_assert(u64(kMaxRun) << kPiece < 1ull << 32 && kFrac - 2 * kPiece <= kPiece, "sums");
+static_assert(kMaxVocab / kMaxCluster + 256 <= kMaxRun, "runs");
 
 __device__ __forceinline__ float sanitize(float v) {
   if (v != v) return 0.f;
@@ -210,25 +212,28 @@ struct Row {
   Queue* queue;
   const ByValue* by_value;  // weights by value (bf16), or null
   int C, rank, turn;    // turn: which slot buffer the next exchange uses
-  int i0, i1;           // this warp's run of indexes
-  bool vec;             // the row starts at a 16-byte boundary
+  int i0, i1;           // this warp's run of indexes (from below 0: see visit)
   bool special;         // it holds NaN or infinities
   float m, dscale;      // maximum; distances from it in second-level bins
   double c, md;         // log2(e) / T; m
 
   static constexpr int VEC = 16 / int(sizeof(T));
   static constexpr int kGroup = 32 * VEC;
+  __device__ __forceinline__ bool inside(int i) const { return uint32_t(i) < uint32_t(i1); }
 
   // f(x, index of x[0]) for this warp's tokens, 32 lanes x 16 bytes at a time, loads three
-  // groups ahead; places past the run hold -infinity, which no token is.  Every lane
-  // makes the same trips.
+  // groups ahead; places outside the run hold -infinity, which no token is.  Every lane
+  // makes the same trips.  Runs begin at 16-byte boundaries: that of a row which does not
+  // begins at the one before it, at an index below 0, and its first group is read token by
+  // token.
   template <typename F>
   __device__ __forceinline__ void visit(F f) const {
     const int first = i0 + int(threadIdx.x & 31) * VEC;
-    const int full = vec ? (i1 - i0) / kGroup : 0, groups = (i1 - i0 + kGroup - 1) / kGroup;
+    const int full = (i1 - i0) / kGroup, groups = (i1 - i0 + kGroup - 1) / kGroup;
+    const auto whole = [&](int g) { return g < full && (g > 0 || i0 >= 0); };
     const uint4* src = reinterpret_cast<const uint4*>(row + first);
     const auto load = [&](int g) -> uint4 {
-      return g < full ? __ldg(src + g * 32) : make_uint4(0, 0, 0, 0);
+      return whole(g) ? __ldg(src + g * 32) : make_uint4(0, 0, 0, 0);
     };
     uint4 r0 = load(0), r1 = load(1), r2 = load(2);
 #pragma unroll 1
@@ -239,18 +244,18 @@ struct Row {
       r2 = load(g + 3);
       const int i = first + g * kGroup;
       float x[VEC];
-      if (g < full) {
+      if (whole(g)) {
         const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) x[j] = Elem<T>::to_f32(e[j]);
       } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) x[j] = i + j < i1 ? Elem<T>::to_f32(row[i + j]) : -INFINITY;
+        for (int j = 0; j < VEC; ++j) x[j] = inside(i + j) ? Elem<T>::to_f32(row[i + j]) : -INFINITY;
       }
       if (special) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
-          x[j] = i + j < i1 ? sanitize(x[j]) : -INFINITY;
+          x[j] = inside(i + j) ? sanitize(x[j]) : -INFINITY;
       }
       f(x, i);
     }
@@ -538,35 +543,34 @@ __device__ __forceinline__ uint32_t unbinned(uint32_t w) {
   return ((mag + kOver * 0x10001u) | ~(mag + kUnder * 0x10001u)) & 0x80008000u;
 }
 
-// f(16 bytes, index of the first token) for a warp's run of a bf16 row, undecoded, loads
-// three groups ahead; places past the run hold -infinity.  Plain arguments, so that
-// nothing of the loop lives in memory.
+// f(16 bytes) for a warp's run of a bf16 row, undecoded, as Row::visit reads it.  Plain
+// arguments, so that nothing of the loop lives in memory.
 template <typename F>
-__device__ __forceinline__ void visit_bf16(const uint16_t* row, int i0, int i1, bool vec, F f) {
+__device__ __forceinline__ void visit_bf16(const uint16_t* row, int i0, int i1, F f) {
   const int first = i0 + int(threadIdx.x & 31) * 8;
-  const int full = vec ? (i1 - i0) / 256 : 0, groups = (i1 - i0 + 255) / 256;
+  const int full = (i1 - i0) / 256, groups = (i1 - i0 + 255) / 256;
+  const auto whole = [&](int g) { return g < full && (g > 0 || i0 >= 0); };
   const uint4* src = reinterpret_cast<const uint4*>(row + first);
   const auto load = [&](int g) -> uint4 {
-    return g < full ? __ldg(src + g * 32) : make_uint4(0, 0, 0, 0);
+    return whole(g) ? __ldg(src + g * 32) : make_uint4(0, 0, 0, 0);
   };
   uint4 r0 = load(0), r1 = load(1), r2 = load(2);
 #pragma unroll 1
-  for (int g = 0; g < full; ++g) {
-    const uint4 raw = r0;
+  for (int g = 0; g < groups; ++g) {
+    uint4 raw = r0;
     r0 = r1;
     r1 = r2;
     r2 = load(g + 3);
-    f(raw, first + g * 256);
-  }
-#pragma unroll 1
-  for (int g = full; g < groups; ++g) {
-    uint32_t w[4] = {0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
-    const int i = first + g * 256;
+    if (!whole(g)) {
+      uint32_t w[4] = {0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
+      const int i = first + g * 256;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (i + j < i1)
-        w[j >> 1] = __byte_perm(w[j >> 1], row[i + j], j & 1 ? 0x5410 : 0x3254);
-    f(make_uint4(w[0], w[1], w[2], w[3]), i);
+      for (int j = 0; j < 8; ++j)
+        if (uint32_t(i + j) < uint32_t(i1))
+          w[j >> 1] = __byte_perm(w[j >> 1], row[i + j], j & 1 ? 0x5410 : 0x3254);
+      raw = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    f(raw);
   }
 }
 
@@ -577,8 +581,8 @@ __device__ __noinline__ Kept sum_above_by_value(Row<__nv_bfloat16> w, float cut)
       reinterpret_cast<const uint8_t*>(w.by_value->weight_positive) - 8 * kValueLo;
   u64 sum = 0;
   uint32_t ties = 0;
-  visit_bf16(reinterpret_cast<const uint16_t*>(w.row), w.i0, w.i1, w.vec,
-             [&](const uint4& raw, int) {
+  visit_bf16(reinterpret_cast<const uint16_t*>(w.row), w.i0, w.i1,
+             [&](const uint4& raw) {
     const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
     const __nv_bfloat162 top = __hmax2(__hmax2(as_bf162(word[0]), as_bf162(word[1])),
                                        __hmax2(as_bf162(word[2]), as_bf162(word[3])));
@@ -613,14 +617,13 @@ __device__ __noinline__ Kept sum_above_by_value(Row<__nv_bfloat16> w, float cut)
 }
 
 // First pass of a bf16 row: counts by value, and the maximum.
-__device__ __noinline__ float count_values(const uint16_t* row, int i0, int i1, bool vec,
-                                           ByValue& bv) {
+__device__ __noinline__ float count_values(const uint16_t* row, int i0, int i1, ByValue& bv) {
   uint8_t* counts = reinterpret_cast<uint8_t*>(bv.positive) - 4 * kValueLo;
   const auto count = [&](uint32_t code) {
     atomicAdd(reinterpret_cast<uint32_t*>(counts + count_offset(code)), 1u);
   };
   __nv_bfloat162 top = __float2bfloat162_rn(-INFINITY);
-  visit_bf16(row, i0, i1, vec, [&](const uint4& raw, int) {
+  visit_bf16(row, i0, i1, [&](const uint4& raw) {
     const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
     const uint32_t odd =
         unbinned(word[0]) | unbinned(word[1]) | unbinned(word[2]) | unbinned(word[3]);
@@ -832,9 +835,9 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
   w.rank = p.C > 1 ? int(cluster_rank()) : 0;
   w.turn = 0;
   w.row = logits + int64_t(r) * p.row_stride;
-  w.vec = (reinterpret_cast<uintptr_t>(w.row) & 15) == 0;
   w.special = false;
-  const int first = min(p.V, w.rank * p.chunk), last = min(p.V, first + p.chunk);
+  const int origin = -int((reinterpret_cast<uintptr_t>(w.row) & 15) / sizeof(T));
+  const int first = min(p.V, origin + w.rank * p.chunk), last = min(p.V, first + p.chunk);
   // every warp owns one run of the CTA's run, in steps of a warp's 512 bytes
   const int per_warp = ((last - first + kWarps - 1) / kWarps + 255) / 256 * 256;
   w.i0 = min(last, first + warp * per_warp);
@@ -854,7 +857,7 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
   // This CTA's run on its way to L2 at once: the passes' own loads are too few in flight
   // to stream it from HBM.  (Whole 16-byte words of the run, 4 KB to a thread.)
   {
-    const uintptr_t lo = (reinterpret_cast<uintptr_t>(w.row + first) + 15) & ~uintptr_t(15);
+    const uintptr_t lo = (reinterpret_cast<uintptr_t>(w.row + max(first, 0)) + 15) & ~uintptr_t(15);
     const uintptr_t hi = reinterpret_cast<uintptr_t>(w.row + last) & ~uintptr_t(15);
     for (uintptr_t a = lo + uintptr_t(t) * 4096; a < hi; a += kThreads * 4096) {
       const uint32_t bytes = uint32_t(min(hi - a, uintptr_t(4096)));
@@ -874,7 +877,7 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
   float mx = -INFINITY;
   uint32_t special = 0;
   if constexpr (kByValue) {
-    mx = count_values(reinterpret_cast<const uint16_t*>(w.row), w.i0, w.i1, w.vec, bv);
+    mx = count_values(reinterpret_cast<const uint16_t*>(w.row), w.i0, w.i1, bv);
   } else {
     w.visit([&](const float(&x)[VEC], int i) {
 #pragma unroll
@@ -882,7 +885,7 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
         mx = fmaxf(mx, x[j]);
         // adding one to the exponent carries into the sign's place when it is all ones
         const uint32_t e = (__float_as_uint(x[j]) & 0x7fffffffu) + 0x00800000u;
-        special |= i + j < w.i1 ? e : 0;
+        special |= w.inside(i + j) ? e : 0;
       }
     });
     special &= 0x80000000u;
@@ -1120,7 +1123,7 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
         if (lane == __ffs(hit) - 1) {
           before += s_inc - sum;
           t_before += n_inc - n;
-          pick(i, min(i + VEC, w.i1));
+          pick(max(i, 0), min(i + VEC, w.i1));
         }
       } else {
         before += __shfl_sync(0xffffffffu, s_inc, 31);
@@ -1145,17 +1148,17 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
 #pragma unroll 1
   for (int i = j0; i < j1; i += VEC) {
     T e[VEC];
-    if (w.vec && i + VEC <= j1) {
+    if (i >= 0 && i + VEC <= j1) {
       const uint4 raw = __ldg(reinterpret_cast<const uint4*>(w.row + i));
       memcpy(e, &raw, 16);
     } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) e[j] = w.row[min(i + j, j1 - 1)];
+      for (int j = 0; j < VEC; ++j) e[j] = w.row[max(0, min(i + j, j1 - 1))];
     }
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       const float x = sanitize(Elem<T>::to_f32(e[j]));
-      if (i + j < j1) {
+      if (uint32_t(i + j) < uint32_t(j1)) {
         n_ties += x == cut;
         if (x > cut) sum += weight(x);
       }
@@ -1163,7 +1166,8 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
   }
   t_before += block_scan(s, n_ties).before;
   before += block_scan(s, sum).before;
-  if (at(before, t_before) <= target && target < at(before + sum, t_before + n_ties)) pick(j0, j1);
+  if (at(before, t_before) <= target && target < at(before + sum, t_before + n_ties))
+    pick(max(j0, 0), j1);
 }
 
 static_assert(sizeof(Queue) <= sizeof(ByValue), "the queue lies over the counts");
@@ -1334,7 +1338,8 @@ extern "C" int as_sample_tokens(int64_t* out, float* logprobs, const void* logit
   p.row_stride = row_stride;
   p.V = vocab;
   p.C = cluster_size(num_rows, vocab);
-  p.chunk = ((vocab + p.C - 1) / p.C + 255) / 256 * 256;
+  const int lead = 16 / dtype_size(dtype) - 1;  // at most: from a boundary to the row
+  p.chunk = ((vocab + lead + p.C - 1) / p.C + 255) / 256 * 256;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   auto run = [&](auto tag) -> int {
     using T = decltype(tag);

@@ -171,6 +171,26 @@ def test_sample_row_strides_and_unaligned_rows():
     check(big[::2, 1:], [0.2, 0.5, 0.8], [1.0] * 3, k=[40] * 3)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("B,V", [(6, 2049), (3, 30001), (160, 33333)])
+def test_sample_rows_from_every_alignment(B, V, dtype):
+    """A base at every place within 16 bytes, rows each from another one (odd strides),
+    the tokens before and behind the rows larger than any of theirs."""
+    for lead in range(128 // torch.finfo(dtype).bits):
+        flat = torch.full((lead + B * (V + 2),), 100.0, dtype=dtype, device=DEV)
+        x = flat[lead:].view(B, V + 2)[:, :V]
+        x.copy_(random_logits(B, V, lead, dtype))
+        n = min(B, 8)
+        g = torch.Generator().manual_seed(lead)
+        u = torch.rand(B, generator=g).tolist()
+        u[0], u[1] = 0.0, 1.0 - 2.0 ** -24
+        check(x, u, [0.9] * B, k=[50, 0] * (B // 2) + [7] * (B % 2), p=[0.95] * B)
+        check(x[:n], u[:n], [1.3] * n)
+        assert torch.equal(ops.sample_tokens(x, rows_of(u, torch.float32),
+                                             rows_of([0.0] * B, torch.float32)),
+                           x.float().argmax(1))
+
+
 def test_sample_frequencies_follow_the_probabilities():
     """Equally spaced u over one row give every kept token its share: the number of the
     N values that fall in a token's interval is off by less than one at either end."""

@@ -11,8 +11,9 @@
 //
 // No sort: every filter keeps a prefix of one order, so a cut (a value, and how many of
 // the tokens equal to it) describes it.  A cut is found by histograms over the distance
-// from the maximum: 1024 bins over 12 nats, then 1024 in the chosen bin, then (rarely)
-// over the values' bits, until one value is left.
+// from the maximum: 1024 bins, then 1024 in the chosen bin, then (rarely) over the values'
+// bits, until one value, or a list short enough to compare each token with all others, is
+// left.
 //
 // Sums decide between neighbouring tokens, and a border token can weigh 1e-6 of the
 // total: weights are computed in 64 bits and summed in fixed point (units of 2^-42 of
@@ -37,7 +38,9 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kBinBits = 10;
 constexpr int kBins = 1 << kBinBits;
-constexpr float kWindow = 12.f;  // nats covered by the first histogram
+constexpr float kWindow = 12.f;  // nats covered by the first histogram of weights
+constexpr float kCountWindow = 24.f;  // units of the logits covered by that of counts
+constexpr int kList = 256;       // tokens left at which a cut is found by comparing them all
 constexpr int kTable = 512;      // 2^(i / 512)
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kMaxRun = (1 << 17) + 256;  // tokens of a CTA
@@ -107,6 +110,10 @@ struct Shared {
   Slot found, found2;
   u64 warp[kWarps];
   int flag;
+  uint32_t n_list;     // tokens left in this CTA's run; the first of them
+  float list[kList];
+  float left[kList];   // the cluster's, and what each measures
+  u64 measure[kList];
 };
 // Tokens waiting for their weight, per warp: one group of a visit past a full batch.
 constexpr int kBatch = 64;
@@ -322,6 +329,7 @@ struct Row {
       sp->kmin[i] = 0xffffffffu;
       sp->kmax[i] = 0;
     }
+    if (threadIdx.x == 0) sp->n_list = 0;
     __syncthreads();
   }
   __device__ __forceinline__ void add(int bin, u64 v) const {
@@ -358,16 +366,19 @@ __device__ __noinline__ Found find(Row<T> w, u64 acc, u64 target, bool keys) {
 #pragma unroll 2
     for (int q = 0; q < C; ++q) {
       const uint32_t from = peer_addr(at, q);
+      // With one bin per thread the second is the first again, and dropped below: loads under
+      // a condition here came out of the compiler with their other value undefined.
       uint32_t h[6];
 #pragma unroll
       for (int e = 0; e < 3; ++e) {
         h[e] = peer_load(from + 4 * kBins * e);
-        h[3 + e] = per == 2 ? peer_load(from + 4 * kBins * e + 4) : 0;
+        h[3 + e] = peer_load(from + 4 * kBins * e + 4 * (per - 1));
       }
       v[0] += h[0] + (u64(h[1]) << kPiece) + (u64(h[2]) << (2 * kPiece));
       v[1] += h[3] + (u64(h[4]) << kPiece) + (u64(h[5]) << (2 * kPiece));
     }
   }
+  if (per == 1) v[1] = 0;
   const Scan sc = block_scan(s, v[0] + v[1]);
   const Slot* all = w.exchange(Slot{sc.total, 0, 0});
   u64 start = acc, whole = acc;
@@ -447,6 +458,8 @@ __device__ __noinline__ Cut select_cut(Row<T> w, bool count, u64 target, float o
         for (int e = 1; e < VEC; ++e) y = e == j ? x[e] : y;
         const u64 v = count ? 1 : (y > over ? w.fixed(y) : 0);
         if (!v) continue;
+        const uint32_t at = atomicAdd(&s.n_list, 1u);
+        if (at < kList) s.list[at] = y;
         const int bin = first ? w.dist(y) & (kBins - 1) : int((hi - ord_key(y)) >> shift);
         w.add(bin, v);
         if (first) {
@@ -455,6 +468,41 @@ __device__ __noinline__ Cut select_cut(Row<T> w, bool count, u64 target, float o
         }
       }
     });
+    __syncthreads();
+    const Slot* all = w.exchange(Slot{s.n_list, 0, 0});
+    uint32_t left = 0;
+    for (int e = 0; e < w.C; ++e) left += uint32_t(all[e].a);
+    if (left <= kList) {
+      // Few: every CTA gathers them, and each token is compared with every other.
+      uint32_t from = 0;
+      for (int e = 0; e < w.C; ++e) {
+        const uint32_t n = uint32_t(all[e].a);
+        if (threadIdx.x < n) {
+          const float y = __uint_as_float(peer_load(peer_addr_of(&s.list[threadIdx.x], e)));
+          s.left[from + threadIdx.x] = y;
+          s.measure[from + threadIdx.x] = count ? 1 : w.fixed(y);
+        }
+        from += n;
+      }
+      __syncthreads();
+      if (threadIdx.x < left) {
+        const float y = s.left[threadIdx.x];
+        u64 above = acc, here = 0;
+#pragma unroll 1
+        for (uint32_t i = 0; i < left; ++i) {
+          const float z = s.left[i];
+          const u64 v = s.measure[i];
+          above += z > y ? v : 0;
+          here += z == y ? v : 0;
+        }
+        if (above < target && above + here >= target)  // equal tokens write the same
+          s.found = Slot{__float_as_uint(y), above, 0};
+      }
+      __syncthreads();
+      hi = ord_key(__uint_as_float(uint32_t(s.found.a)));
+      acc = s.found.b;
+      break;
+    }
     const int b1 = f.bin;
     f = find(w, acc, target, first);
     w.turn ^= 1;
@@ -955,7 +1003,7 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
   const double T64 = double(T_);
   w.c = 1.4426950408889634 / T64;
   w.md = double(m);
-  w.dscale = float(double(1 << (2 * kBinBits)) / double(kWindow) / T64);
+  w.dscale = float(1 << (2 * kBinBits)) / kCountWindow;
 
   float cut = -INFINITY;  // everything is above it
   u64 ties = ~0ull;
@@ -995,6 +1043,7 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
       ties = u64(k) - c.above;
     }
     if (by_p) {
+      w.dscale = float(double(1 << (2 * kBinBits)) / double(kWindow) / T64);
       // weights of the first n_k: all above the cut, and `ties` times the weight at it
       const Kept kept = sum_above(w, cut, true);
       all = w.exchange(Slot{block_scan(s, lane == 0 ? kept.sum : 0).total, 0, 0});

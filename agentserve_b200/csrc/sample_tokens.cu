@@ -25,6 +25,7 @@
 #include <stddef.h>
 #include <string.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -86,6 +87,13 @@ __device__ __forceinline__ uint32_t peer_load(uint32_t addr) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
   return v;
 }
+__device__ __forceinline__ uint4 peer_load4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr));
+  return v;
+}
 __device__ __forceinline__ void peer_store64(uint32_t addr, u64 v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
@@ -102,7 +110,7 @@ __device__ __forceinline__ void cluster_sync(int C) {
 struct Slot {
   u64 a, b, c;
 };
-struct Shared {
+struct alignas(16) Shared {
   double table[kTable];       // 2^(i / 512) in units of the fixed point
   uint32_t hist[3][kBins];    // pieces of the summed measure
   uint32_t kmin[kBins], kmax[kBins];
@@ -121,6 +129,7 @@ constexpr int kQueue = kBatch - 1 + 256;
 struct Queue {
   float x[kWarps][kQueue + 1];
 };
+static_assert(sizeof(Queue) >= 3 * kBins * 4 && kThreads == kBins / 2, "find() stages over it");
 
 // bf16 rows: a histogram by value.  The 4096 values of magnitude 2^-9 to 128 have a
 // bin each; the few closer to zero are listed; those at or below -128 (masks) weigh
@@ -359,26 +368,32 @@ __device__ __noinline__ Found find(Row<T> w, u64 acc, u64 target, bool keys) {
   const int C = w.C, t = threadIdx.x;
   cluster_sync(C);  // every CTA's histogram is complete
   const int S = kBins / C;  // bins of this CTA's slice; thread t has 2t, 2t + 1 or t
-  const int per = S > kThreads ? 2 : 1, bin0 = w.rank * S + t * per;
-  u64 v[2] = {0, 0};
-  if (t * per < S) {
-    const uint32_t at = smem_u32(&s.hist[0][bin0]);
-#pragma unroll 2
-    for (int q = 0; q < C; ++q) {
-      const uint32_t from = peer_addr(at, q);
-      // With one bin per thread the second is the first again, and dropped below: loads under
-      // a condition here came out of the compiler with their other value undefined.
-      uint32_t h[6];
-#pragma unroll
-      for (int e = 0; e < 3; ++e) {
-        h[e] = peer_load(from + 4 * kBins * e);
-        h[3 + e] = peer_load(from + 4 * kBins * e + 4 * (per - 1));
-      }
-      v[0] += h[0] + (u64(h[1]) << kPiece) + (u64(h[2]) << (2 * kPiece));
-      v[1] += h[3] + (u64(h[4]) << kPiece) + (u64(h[5]) << (2 * kPiece));
+  const int per = S > kThreads ? 2 : 1, mine = t * per, bin0 = w.rank * S + mine;
+  const uint32_t* from = &s.hist[0][0];
+  if (C > 1) {
+    // The slice of every CTA's three histograms, side by side, over the queue (not in use
+    // now): 768 loads of 16 bytes, all in flight at once.  (Summed straight from the peers,
+    // three words at a time: find() took 11.5K cycles of a call's 47K.)
+    uint32_t* stage = reinterpret_cast<uint32_t*>(w.queue);
+    const int r = (t & (kBins / 4 - 1)) * 4, e = t / (kBins / 4);  // e: 0 or 1
+    const uint32_t at = peer_addr_of(&s.hist[0][w.rank * S + (r & (S - 1))], r / S);
+    const uint4 x = peer_load4(at + 4 * kBins * e);
+    if (e == 0) {
+      const uint4 y = peer_load4(at + 4 * kBins * 2);
+      *reinterpret_cast<uint4*>(stage + 2 * kBins + r) = y;
     }
+    *reinterpret_cast<uint4*>(stage + kBins * e + r) = x;
+    from = stage;
+    __syncthreads();
   }
-  if (per == 1) v[1] = 0;
+  u64 v[2] = {0, 0};
+  if (mine < S) {
+    const auto bin = [&](const uint32_t* h) -> u64 {
+      return h[0] + (u64(h[kBins]) << kPiece) + (u64(h[2 * kBins]) << (2 * kPiece));
+    };
+    for (int q = 0; q < C; ++q) v[0] += bin(from + q * S + mine);
+    if (per == 2) v[1] = bin(from + mine + 1);  // C = 1
+  }
   const Scan sc = block_scan(s, v[0] + v[1]);
   const Slot* all = w.exchange(Slot{sc.total, 0, 0});
   u64 start = acc, whole = acc;
@@ -1149,8 +1164,9 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
       }
     }
   };
-  if (per_warp <= 2048) {
-    // a short run: the warp whose it is walks it, 32 lanes x 16 bytes at a time
+  if (per_warp <= 512) {
+    // A short run: the warp whose it is walks it, 32 lanes x 16 bytes at a time.  (Runs of 2048
+    // walked so: 64 bf16 rows of 128256 tokens 42 us instead of 36, fp32 100 instead of 88.)
     if (!__shfl_sync(0xffffffffu, ahead <= target && target < after, 0)) return;
     before = __shfl_sync(0xffffffffu, before, 0);
     t_before = __shfl_sync(0xffffffffu, t_before, 0);
@@ -1343,13 +1359,61 @@ sample_small_kernel(const T* __restrict__ logits, const Params p) {
   }
 }
 
-// CTAs of a row's cluster: enough to fill the SMs (two CTAs each) when rows are few, at
-// least 2048 tokens each so that the exchanges do not outweigh the work, and never more
-// than kMaxRun each.
+template <typename T>
+cudaLaunchConfig_t launch_config(int clusters, int C, cudaLaunchAttribute* attr,
+                                 cudaStream_t stream = nullptr) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(clusters) * C);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cfg.dynamicSmemBytes = std::is_same<T, __nv_bfloat16>::value ? sizeof(ByValue) : sizeof(Queue);
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = C;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = C > 1 ? 2 : 1;
+  return cfg;
+}
+
+// Clusters of C CTAs that the device holds at once, asked for once (148 SMs: 148 of 2, 71 of
+// 4, 33 of 8; fewer than the CTAs' own 296 would give).
+template <typename T>
+int resident_clusters(int C) {
+  constexpr int kDevices = 64;
+  static std::atomic<int> known[kDevices][kMaxCluster + 1];
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  if (dev < kDevices && (n = known[dev][C].load(std::memory_order_relaxed)) > 0) return n;
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg = launch_config<T>(1, C, attr);
+  if (cudaOccupancyMaxActiveClusters(&n, sample_tokens_kernel<T>, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (dev < kDevices) known[dev][C].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// CTAs of a row's cluster: as many as leave the rows' clusters all resident, with at least
+// 2048 tokens each so that the exchanges do not outweigh the work, and at most kMaxRun.
+// Rows in bf16, whose passes are short, keep an SM to each CTA.  Measured, us, top-p 0.9:
+//   rows x tokens           C = 1   2    4    8
+//   fp32  14 x 128256       188   107   64   43
+//   fp32  36 x 128256       188   106   86   92
+//   fp32  72 x 128256       188   107  133  145
+//   bf16  14 x 128256        51    34   24   19
+//   bf16  24 x 32003         24    19   17   18
+//   bf16  64 x 128256        52    34   37   52
+//   bf16 148 x 32003         25    26   50   79
+template <typename T>
 int cluster_size(int rows, int vocab) {
+  const int share = std::is_same<T, __nv_bfloat16>::value ? 2 : 1;
   int c = 1;
   while (c < kMaxCluster &&
-         ((int64_t(rows) * c * 2 <= 2 * int64_t(sm_count()) && vocab / (2 * c) >= 2048) ||
+         ((vocab / (2 * c) >= 2048 && int64_t(rows) * share <= resident_clusters<T>(2 * c)) ||
           (vocab + c - 1) / c > kMaxRun - 256))
     c *= 2;
   return c;
@@ -1386,9 +1450,6 @@ extern "C" int as_sample_tokens(int64_t* out, float* logprobs, const void* logit
   p.min_p = min_p;
   p.row_stride = row_stride;
   p.V = vocab;
-  p.C = cluster_size(num_rows, vocab);
-  const int lead = 16 / dtype_size(dtype) - 1;  // at most: from a boundary to the row
-  p.chunk = ((vocab + lead + p.C - 1) / p.C + 255) / 256 * 256;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   auto run = [&](auto tag) -> int {
     using T = decltype(tag);
@@ -1399,22 +1460,14 @@ extern "C" int as_sample_tokens(int64_t* out, float* logprobs, const void* logit
                  sizeof(SmallShared), s, static_cast<const T*>(logits), p);
       return check_launch("as_sample_tokens");
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(num_rows) * p.C);
-    cfg.blockDim = dim3(kThreads);
-    cfg.stream = s;
-    cfg.dynamicSmemBytes = std::is_same<T, __nv_bfloat16>::value ? sizeof(ByValue) : sizeof(Queue);
-    cudaFuncSetAttribute(sample_tokens_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         int(cfg.dynamicSmemBytes));
+    cudaFuncSetAttribute(
+        sample_tokens_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        int(std::is_same<T, __nv_bfloat16>::value ? sizeof(ByValue) : sizeof(Queue)));
+    p.C = cluster_size<T>(num_rows, vocab);
+    const int lead = 16 / int(sizeof(T)) - 1;  // at most: from a boundary to the row
+    p.chunk = ((vocab + lead + p.C - 1) / p.C + 255) / 256 * 256;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = p.C;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = p.C > 1 ? 2 : 1;
+    const cudaLaunchConfig_t cfg = launch_config<T>(num_rows, p.C, attr, s);
     cudaLaunchKernelEx(&cfg, sample_tokens_kernel<T>, static_cast<const T*>(logits), p);
     return check_launch("as_sample_tokens");
   };

@@ -40,23 +40,24 @@ constexpr float kLazySlack = 8.0f;  // log2 units a row's scores may exceed its 
 template <int HD>
 struct PreCfg {
   static constexpr int D = HD;
-  static constexpr int kBN = 128;                 // keys per tile
+  static constexpr int kBN = D == 64 ? 128 : 64;  // keys per tile
   static constexpr int kBlocks = kBN / kBS;
   static constexpr int kSub = D / 64;             // 128-byte-wide swizzle sub-tiles
   static constexpr int kQSub = 128 * 128;
   static constexpr int kKVSub = kBN * 128;
   static constexpr int kQBytes = kSub * kQSub;    // 128 rows
   static constexpr int kKVBytes = kSub * kKVSub;  // K (or V) of one tile
-  static constexpr int kStages = D == 64 ? 4 : 2;  // even: a stage always serves one stream
+  static constexpr int kStages = 4;  // even: a stage always serves one stream
   static constexpr int kOffKV = 2 * kQBytes;
   static constexpr int kOffBar = kOffKV + kStages * 2 * kKVBytes;
   static constexpr int kSmemBytes = kOffBar + 256;
   static constexpr int kThreads = 320;
-  // TMEM columns of a stream, from 256 i: S [0, 128), P (16-bit pairs), O the last D.  At
-  // D = 128 they do not fit side by side: P overwrites S, already in registers, and
-  // S(j+1) is issued after PV(j), which reads P, in the MMA thread's order.
+  // TMEM columns of a stream, from 256 i: S, P (16-bit pairs), O the last D.  At D = 128
+  // two S of 64 keys take turns, so that the next one is ready when a softmax ends, and P
+  // overwrites the S it came from, by then in registers.  (One S of 128 keys under its P,
+  // the next issued after PV: 256 sequences on 30,000 tokens 227 us instead of 209.)
   static constexpr int kCols = 512;
-  static constexpr bool kAliasP = kBN + kBN / 2 > 256 - D;
+  static constexpr bool kAliasP = D == 128;
   static constexpr int kColP = kAliasP ? 0 : kBN;
   static constexpr int kColO = 256 - D;
   static_assert(kSmemBytes + 1024 <= 227 * 1024, "shared memory");
@@ -64,7 +65,7 @@ struct PreCfg {
 
 struct PreBars {
   uint64_t kv_full[4], kv_empty[4];
-  uint64_t s_full[2], s_free[2], p_full[2], pv_done[2];
+  uint64_t s_full[2][2], s_free[2], p_full[2], pv_done[2];  // [stream], S's place
   uint64_t turn[2][4];  // hand-off of the exponent unit between a sub-partition's warps
   uint64_t drain;
   uint32_t tmem;
@@ -113,7 +114,8 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
     }
     for (int i = 0; i < 2; ++i) {
       const int n = max(1, i ? active1 : active0);
-      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->s_full[i][0], 1);
+      mbar_init(&bars->s_full[i][1], 1);
       mbar_init(&bars->s_free[i], n);
       mbar_init(&bars->p_full[i], n);
       mbar_init(&bars->pv_done[i], 1);
@@ -221,22 +223,24 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
 
   if (warp == 1) {
     // ----------------------------------------------------------------- MMAs
-    if (lane == 0) {
-      auto issue_s = [&](int i, int st) {
+    // An MMA costs this thread 20 cycles; under a branch on lane == 0 it cost 77, and the
+    // issue bound the launch (256 sequences on 30,000 tokens 243 us instead of 209).
+    if (tc::elect_one()) {
+      auto issue_s = [&](int i, int st, int place) {
         const uint32_t qi = sQ + (halves ? 0 : i) * Cfg::kQBytes;
         const uint32_t k = sKV + st * 2 * Cfg::kKVBytes;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          tc::mma_f16(tmem + 256 * i,
+          tc::mma_f16(tmem + 256 * i + place * BN,
                       tc::sdesc_sw128(qi + (kk >> 2) * Cfg::kQSub + (kk & 3) * 32, 16, 1024),
                       tc::sdesc_sw128(k + (kk >> 2) * Cfg::kKVSub + (kk & 3) * 32, 16, 1024),
                       kIdescS, kk > 0 ? 1u : 0u);
       };
-      auto issue_pv = [&](int i, int st, bool acc) {
+      auto issue_pv = [&](int i, int st, int place, bool acc) {
         const uint32_t v = sKV + st * 2 * Cfg::kKVBytes + Cfg::kKVBytes;
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
-          tc::mma_f16_ts(tmem + 256 * i + Cfg::kColO, tmem + 256 * i + Cfg::kColP + kk * 8,
+          tc::mma_f16_ts(tmem + 256 * i + Cfg::kColO, tmem + 256 * i + Cfg::kColP + place * BN + kk * 8,
                          tc::sdesc_sw128(v + kk * 2048, Cfg::kKVSub, 1024), kIdescO,
                          (acc || kk > 0) ? 1u : 0u);
       };
@@ -252,20 +256,21 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
         for (int i = 0; i < 2; ++i) {
           const int j = js[i];
           const int t = stride * j + odd * i;
-          if (j < nk[i] && (!Cfg::kAliasP || jp[i] >= j) &&
-              mbar_try_wait(&bars->kv_full[t % NS], (t / NS) & 1) &&
-              (j == 0 || mbar_try_wait(&bars->s_free[i], (j - 1) & 1))) {
+          const int place = Cfg::kAliasP ? j & 1 : 0;
+          if (j < nk[i] && mbar_test_wait(&bars->kv_full[t % NS], (t / NS) & 1) &&
+              (Cfg::kAliasP ? jp[i] >= j - 1  // PV(j - 2), which reads P there, is issued
+                            : j == 0 || mbar_test_wait(&bars->s_free[i], (j - 1) & 1))) {
             tc::fence_after_sync();
-            issue_s(i, t % NS);
-            tc::commit(&bars->s_full[i]);
+            issue_s(i, t % NS, place);
+            tc::commit(&bars->s_full[i][place]);
             js[i] = j + 1;
             did = true;
           }
           const int jq = jp[i];
-          if (jq < js[i] && mbar_try_wait(&bars->p_full[i], jq & 1)) {
+          if (jq < js[i] && mbar_test_wait(&bars->p_full[i], jq & 1)) {
             const int tq = stride * jq + odd * i;
             tc::fence_after_sync();
-            issue_pv(i, tq % NS, jq > 0);
+            issue_pv(i, tq % NS, Cfg::kAliasP ? jq & 1 : 0, jq > 0);
             tc::commit(&bars->pv_done[i]);
             jp[i] = jq + 1;
             did = true;
@@ -298,14 +303,17 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
     const int r = quad * 32 + lane;
     const int my_rows = i ? rows1 : rows0, n = i ? n1 : n0;
     if (quad < (i ? active1 : active0)) {
-      const uint32_t tS = tmem + 256 * i + (uint32_t(quad * 32) << 16);
-      const uint32_t tP = tS + Cfg::kColP, tO = tS + Cfg::kColO;
+      const uint32_t row = tmem + 256 * i + (uint32_t(quad * 32) << 16);
+      const uint32_t tO = row + Cfg::kColO;
       const bool partner = quad < (i ? active0 : active1);
       float m = -INFINITY, l = 0.f;
       bool ok = true;
       for (int j = 0; j < n; ++j) {
+        const int place = Cfg::kAliasP ? j & 1 : 0;
+        const uint32_t tS = row + place * BN, tP = tS + Cfg::kColP;
         const bool go = !stopped(abort_flag) &&
-                        mbar_wait(&bars->s_full[i], j & 1, a.status, a.wait_limit);
+                        mbar_wait(&bars->s_full[i][place], (Cfg::kAliasP ? j >> 1 : j) & 1,
+                                  a.status, a.wait_limit);
         if (!__all_sync(0xffffffffu, go)) {
           ok = false;
           break;
@@ -322,9 +330,11 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
 #pragma unroll
             for (int c = 0; c < 32; ++c) x[32 * u + c] = __uint_as_float(v[u][c]);
         }
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->s_free[i]);
+        if (!Cfg::kAliasP) {
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->s_free[i]);
+        }
         const int keys = (it.end - it.begin) * kBS - (stride * j + odd * i) * BN;  // of this tile
         if (keys < BN) {
 #pragma unroll
@@ -448,14 +458,16 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
 // ===========================================================================
 template <int D>
 struct OwnCfg {
-  static constexpr int kWarps = 4;  // consumers; one more warp loads
+  // Consumers; one more warp loads.  At D = 128 three and one stage, so that a block fits
+  // beside one of the prefix launch (four and two: 209 us instead of 201, as above).
+  static constexpr int kWarps = D == 64 ? 4 : 3;
   static constexpr int kThreads = (kWarps + 1) * 32;
   static constexpr int kSub = D / 64;
   static constexpr int kSubBytes = kBS * 128;
   static constexpr int kTileBytes = kSub * kSubBytes;  // one block of K or V, one head
   static constexpr int kSlotBytes = 2 * kTileBytes;
   static constexpr int kStageBytes = kWarps * kSlotBytes;  // a block per consumer warp
-  static constexpr int kStages = D == 64 ? 3 : 2;
+  static constexpr int kStages = D == 64 ? 3 : 1;
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 2 * kStages * 8;
   static constexpr int kHeads = 8;
   static constexpr int kJoinFloats = kWarps * kHeads * (D + 2);

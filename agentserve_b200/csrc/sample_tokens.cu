@@ -107,6 +107,19 @@ __device__ __forceinline__ void cluster_sync(int C) {
   }
 }
 
+// The two halves of a first barrier: a CTA's shared memory may be written by others once it
+// runs.
+__device__ __forceinline__ void cluster_started(int C) {
+  if (C == 1) return;
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait_started(int C) {
+  if (C == 1) return;
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 struct Slot {
   u64 a, b, c;
 };
@@ -138,7 +151,8 @@ static_assert(sizeof(Queue) >= 3 * kBins * 4 && kThreads == kBins / 2, "find() s
 // weights up.  Rows outside this (values of 128 and more, NaN, cuts among the listed
 // values, u <= 0) take the general path.
 //
-// The passes are bound by integer instructions (half rate), so a value's place is two
+// 64 rows of 128,256 tokens, top-p: 34 us, and 83 by the general path (fp16).  The passes
+// are bound by integer instructions (half rate), so a value's place is two
 // logic operations and a multiply-add away from its 16 bits: counts (4 bytes each) and
 // weights (8) lie in ascending magnitude, those of the negative values 0x8000 bytes after
 // those of the positive ones.
@@ -906,6 +920,7 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
   w.i0 = min(last, first + warp * per_warp);
   w.i1 = min(last, w.i0 + per_warp);
 
+  cluster_started(p.C);
   if (t == 0) s.flag = 0;
   for (int i = t; i < kTable; i += kThreads)
     s.table[i] = exp2(double(i) / kTable) * double(1ull << kFrac);
@@ -966,6 +981,7 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
   };
   mine.a = block_max(ord_key(mx), special != 0);
   if (kByValue && (bv.refuse || !(u > 0.f))) mine.a |= 1ull << 32;
+  cluster_wait_started(p.C);
   const Slot* all = w.exchange(mine);
   uint32_t top = 0;
   for (int q = 0; q < p.C; ++q) {
@@ -1238,8 +1254,9 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
 static_assert(sizeof(Queue) <= sizeof(ByValue), "the queue lies over the counts");
 
 // Rows of at most kSmall tokens: one CTA sorts (value descending, index ascending), and
-// every filter is a length of the sorted row.
-constexpr int kSmall = 2048;
+// every filter is a length of the sorted row.  Against the clusters, 64 rows, top-k and
+// top-p: 256 tokens 7 us (bf16 15, fp32 21), 1,000 13 (16, 20), 2,048 23 (15, 20).
+constexpr int kSmall = 1024;
 struct SmallShared {
   Shared s;  // block_scan's
   u64 key[kSmall];
@@ -1453,7 +1470,7 @@ extern "C" int as_sample_tokens(int64_t* out, float* logprobs, const void* logit
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   auto run = [&](auto tag) -> int {
     using T = decltype(tag);
-    if (vocab <= kSmall) {  // a sort costs less than the histograms' exchanges
+    if (vocab <= kSmall) {
       cudaFuncSetAttribute(sample_small_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            int(sizeof(SmallShared)));
       launch_pdl(sample_small_kernel<T>, dim3(unsigned(num_rows)), dim3(kThreads),

@@ -64,7 +64,7 @@ sp_generic_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
   const int D = a.D, group = a.group;
 
   // this item's query rows and token range
-  int b = 0, split = 0, row0, rows, begin, end, part = 0, step = 0, table_row;
+  int b = 0, split = 0, row0, rows, begin, end, part = 0, table_row;
   const int32_t* members = nullptr;
   RowPlan rp{};
   if (kPrefix) {
@@ -76,7 +76,6 @@ sp_generic_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
     begin = it.begin * kBS;
     end = it.end * kBS;
     part = it.part;
-    step = it.step;
     table_row = it.table_row;
   } else {
     const OwnItem it = load_item(a.own_items, blockIdx.x);
@@ -229,8 +228,6 @@ sp_generic_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
       a.parts.o[at * D + d] = ro[r * DP + d];
       if (d == 0) {
         a.parts.ml[at] = make_float2(rm[r], rl[r]);
-        // one part holds both halves of the keys here
-        if (step > 0) a.parts.ml[at + size_t(step) * a.H] = make_float2(-INFINITY, 0.f);
       }
     }
     return;
@@ -241,10 +238,15 @@ sp_generic_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
 }
 
 constexpr int kGenericRows = 32;
-// Fixed costs of a block, in the units of its piece: 128-key softmax passes, and blocks.
+// Fixed costs of a block, in the units of its piece: halves of a 128-key tile, and blocks of
+// 16 keys.  Measured, us per call (n sequences on their shared tokens): prefix 5, with 2 the
+// same everywhere, with 10 256 on 30,000 249 instead of 203; own 16, with 32 the same, with
+// 6 64 on 4,096 28 instead of 21 and on 14,336 40 instead of 34.
 constexpr int64_t kPrefixOverhead = 5;
 constexpr int64_t kOwnOverhead = 16;
-constexpr int64_t kMinOwn = 8;  // blocks: two per consumer warp
+// Least own blocks of an item, where a row has that many: with 4, 16 fp32 sequences on 1,024
+// take 34 us instead of 27; with 16 as with 8.
+constexpr int64_t kMinOwn = 8;
 
 template <typename T, int DP, int RW, int TG, bool kPrefix>
 int launch_generic_one(dim3 grid, int tile_rows, T* out, const T* q, const T* k, const T* v, const Args& a,
@@ -312,7 +314,7 @@ Limits limits(int B, int H, int Kh, int D, int dtype) {
   n.prefix_items = 2 * n.prefix_slots / Kh + tiles;
   n.own_items = 4 * n.own_slots / n.own_per_item + B;
   // a prefix CTA leaves at most tile_rows rows of parts
-  n.prefix_parts = 2 * int64_t(B) + 2 * int64_t(n.prefix_slots) * n.tile_rows / H;
+  n.prefix_parts = int64_t(B) + 2 * int64_t(n.prefix_slots) * n.tile_rows / H;
   n.own_parts = n.own_items;
   return n;
 }
@@ -398,8 +400,6 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
   try {
     struct Group {
       int first, size, blocks, tiles, tile_rows, splits, chunk;
-      int64_t cost;  // of a 128-key tile, in softmax passes over 128 rows
-      bool halves;   // one tile of at most 128 rows: two halves of the keys side by side
     };
     std::vector<Group> groups;
     std::vector<int> shared(B, 0), seen(B, 0);
@@ -423,38 +423,27 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
       }
       // one member, or nothing shared: its keys are its own
       if (hi - lo < 2 || prefix_blocks[i] == 0) continue;
-      // Whole members to a tile.  On tensor cores a pass over 256 rows costs twice one
-      // over 128, so a rest of at most 128 rows is a group of its own, at half the cost.
-      const int per_tile = std::max(1, n.tile_rows / group);
-      const int full = (hi - lo) / per_tile * per_tile;
-      for (int first = lo; first < hi;) {
-        const int size = n.tc && first == lo && full > 0 ? full : hi - first;
-        Group g{int(list.size()), size, prefix_blocks[i], 0, 0, 0, 0, 1, false};
-        const int rows = size * group;
-        g.tile_rows = group > n.tile_rows ? n.tile_rows : per_tile * group;
-        g.tiles = (rows + g.tile_rows - 1) / g.tile_rows;
-        if (n.tc) {
-          g.halves = rows <= n.tile_rows / 2;
-          g.cost = g.halves ? 1 : 2;
-        }
-        for (int j = first; j < first + size; ++j) {
-          list.push_back(members[j]);
-          shared[members[j]] = g.blocks;
-        }
-        groups.push_back(g);
-        first += size;
+      // whole members to a tile
+      Group g{int(list.size()), hi - lo, prefix_blocks[i], 0, 0, 0, 0};
+      g.tile_rows = group > n.tile_rows ? n.tile_rows : n.tile_rows / group * group;
+      g.tiles = (g.size * group + g.tile_rows - 1) / g.tile_rows;
+      for (int j = lo; j < hi; ++j) {
+        list.push_back(members[j]);
+        shared[members[j]] = g.blocks;
       }
+      groups.push_back(g);
     }
     for (int b = 0; b < B; ++b)
       if (row_blocks[b] < 0) return fail(AS_ERR_INVALID_ARG, "%s: negative row_blocks", who);
 
-    // prefix splits: pieces of about equal cost, in units of 8 blocks
+    // prefix splits: pieces of about equal length, in units of 8 blocks (half units on
+    // tensor cores, for the fixed cost)
+    const int64_t cost = n.tc ? 2 : 1;
     auto split_prefix = [&](int64_t piece) -> int64_t {
       int64_t ctas = 0;
       for (Group& g : groups) {
         const int units = (g.blocks + 7) / 8;
-        const int most = kMaxSplits / (g.halves ? 2 : 1);
-        const int splits = int(std::min<int64_t>(most, (units * g.cost + piece - 1) / piece));
+        const int splits = int(std::min<int64_t>(kMaxSplits, (units * cost + piece - 1) / piece));
         g.chunk = (units + splits - 1) / splits * 8;
         g.splits = (g.blocks + g.chunk - 1) / g.chunk;
         ctas += int64_t(g.splits) * g.tiles * Kh;
@@ -463,13 +452,13 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
     };
     if (!groups.empty()) {
       int64_t most = 2;
-      for (const Group& g : groups) most = std::max(most, (g.blocks + 7) / 8 * g.cost);
+      for (const Group& g : groups) most = std::max(most, (g.blocks + 7) / 8 * cost);
       int64_t piece = best_piece(n.tc ? 2 : 1, most, n.prefix_slots, 2, n.tc ? kPrefixOverhead : 1,
                                  split_prefix);
       for (;; piece += (piece + 1) / 2) {  // and within the workspace's parts and the items
         const int64_t ctas = split_prefix(piece);
         int64_t parts = 0;
-        for (const Group& g : groups) parts += int64_t(g.splits) * g.size * (g.halves ? 2 : 1);
+        for (const Group& g : groups) parts += int64_t(g.splits) * g.size;
         if (parts <= n.prefix_parts && ctas / Kh <= n.prefix_items) break;
       }
     }
@@ -498,12 +487,11 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
     int n_pre = 0, n_own = 0, most = 0;
     int part = 0;
     for (const Group& g : groups) {
-      const int ways = g.halves ? 2 : 1;
       most = std::max(most, g.blocks);
       for (int i = 0; i < g.size; ++i) {
         OwnItem& r = row_items[list[g.first + i]];
         r.shared = g.blocks;
-        r.prefix_splits = g.splits * ways;
+        r.prefix_splits = g.splits;
         r.prefix_part = part + i;
         r.prefix_step = g.size;
       }
@@ -517,10 +505,9 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
           it.rows = std::min(g.tile_rows, all_rows - t * g.tile_rows);
           it.begin = s * g.chunk;
           it.end = std::min(g.blocks, (s + 1) * g.chunk);
-          it.part = part + s * ways * g.size;
-          it.step = g.halves ? g.size : 0;
+          it.part = part + s * g.size;
         }
-      part += g.splits * ways * g.size;
+      part += g.splits * g.size;
     }
     // own items, the longest first so that the last to start are short
     std::vector<std::pair<int64_t, OwnItem>> items;

@@ -32,7 +32,7 @@ struct PrefixItem {
   int row0, rows; // query rows (member, head of the KV head) of the group
   int begin, end; // blocks
   int part;       // part index of the group's first member (a part holds H heads)
-  int step;       // > 0: two halves of the keys go to parts `step` apart
+  int unused;     // 0
 };
 struct OwnItem {
   int row, split;     // batch row, and which of its own_splits ranges

@@ -2,9 +2,8 @@
 //
 // Prefix launch (sp_prefix_kernel).  A group's members' query heads of KV head g are the
 // rows of a matrix that attends over the shared blocks.  A block runs two softmax
-// streams of 128 rows: the two halves of a tile of up to 256 rows, which share every
-// K / V tile, or, for a group of at most 128 rows, the same rows twice over the even
-// and the odd key tiles.  S = Q K^T by tcgen05.mma into TMEM, P back into TMEM as the A
+// streams of 128 rows, the two halves of a tile of up to 256 rows, which share every
+// K / V tile.  S = Q K^T by tcgen05.mma into TMEM, P back into TMEM as the A
 // operand of O += P V; K / V arrive by TMA, paged block by paged block.  Roles (320
 // threads, one block per SM): warp 0 loads K / V, warp 1 issues MMAs by polling which
 // stream is ready, warps 2-5 and 6-9 the streams' softmax, one row per thread, the two
@@ -47,7 +46,7 @@ struct PreCfg {
   static constexpr int kKVSub = kBN * 128;
   static constexpr int kQBytes = kSub * kQSub;    // 128 rows
   static constexpr int kKVBytes = kSub * kKVSub;  // K (or V) of one tile
-  static constexpr int kStages = 4;  // even: a stage always serves one stream
+  static constexpr int kStages = 4;
   static constexpr int kOffKV = 2 * kQBytes;
   static constexpr int kOffBar = kOffKV + kStages * 2 * kKVBytes;
   static constexpr int kSmemBytes = kOffBar + 256;
@@ -98,13 +97,9 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
   if (it.rows == 0) return;
   const int g = blockIdx.y, group = a.group;
   const int n_tiles = (it.end - it.begin + NB - 1) / NB;
-  const bool halves = it.step > 0;
-  // streams: rows and key tiles of each; stream i's tile j is key tile stride * j + i * odd
-  const int rows0 = min(it.rows, 128);
-  const int rows1 = halves ? rows0 : it.rows - rows0;
-  const int stride = halves ? 2 : 1, odd = halves ? 1 : 0;
-  const int n0 = halves ? (n_tiles + 1) / 2 : n_tiles;
-  const int n1 = halves ? n_tiles / 2 : (rows1 > 0 ? n_tiles : 0);
+  // streams: rows and key tiles of each
+  const int rows0 = min(it.rows, 128), rows1 = it.rows - rows0;
+  const int n0 = n_tiles, n1 = rows1 > 0 ? n_tiles : 0;
   const int active0 = (rows0 + 31) / 32, active1 = (rows1 + 31) / 32;  // warps with rows
 
   if (threadIdx.x == 0) {
@@ -182,11 +177,9 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
     tc::tmem_alloc(&bars->tmem, Cfg::kCols);
     tc::tmem_relinquish();
   } else if (warp >= 2) {
-    // Q rows (member, head) into the 128B-swizzled layout, a thread per row or half row,
-    // all copies in flight at once; rows past a tile are zero
-    const int t = threadIdx.x - 64;
-    const int r = halves ? t & 127 : t;
-    const int c0 = halves && t >= 128 ? D / 16 : 0, c1 = halves && t < 128 ? D / 16 : D / 8;
+    // Q rows (member, head) into the 128B-swizzled layout, a thread per row, all
+    // copies in flight at once; rows past a tile are zero
+    const int r = threadIdx.x - 64;
     uint8_t* dst = smem + (r >> 7) * Cfg::kQBytes + (r & 127) * 128;
     const auto chunk = [&](int c) -> uint8_t* {
       return dst + (c >> 3) * Cfg::kQSub + (((c & 7) ^ (r & 7)) << 4);
@@ -197,10 +190,10 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
                      int64_t(g * group + rr % group) * D;
       if (((reinterpret_cast<uintptr_t>(q) | uintptr_t(a.q_stride * 2)) & 15) == 0) {
 #pragma unroll 4
-        for (int c = c0; c < c1; ++c) cp_async_16(smem_u32(chunk(c)), src + c * 8);
+        for (int c = 0; c < D / 8; ++c) cp_async_16(smem_u32(chunk(c)), src + c * 8);
         asm volatile("cp.async.wait_all;" ::: "memory");
       } else {
-        for (int c = c0; c < c1; ++c) {
+        for (int c = 0; c < D / 8; ++c) {
           T e[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) e[j] = src[c * 8 + j];
@@ -208,7 +201,7 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
         }
       }
     } else {
-      for (int c = c0; c < c1; ++c) *reinterpret_cast<uint4*>(chunk(c)) = make_uint4(0, 0, 0, 0);
+      for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(chunk(c)) = make_uint4(0, 0, 0, 0);
     }
     fence_proxy_async_smem();
   }
@@ -227,7 +220,7 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
     // issue bound the launch (256 sequences on 30,000 tokens 243 us instead of 209).
     if (tc::elect_one()) {
       auto issue_s = [&](int i, int st, int place) {
-        const uint32_t qi = sQ + (halves ? 0 : i) * Cfg::kQBytes;
+        const uint32_t qi = sQ + i * Cfg::kQBytes;
         const uint32_t k = sKV + st * 2 * Cfg::kKVBytes;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
@@ -255,27 +248,25 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int j = js[i];
-          const int t = stride * j + odd * i;
           const int place = Cfg::kAliasP ? j & 1 : 0;
-          if (j < nk[i] && mbar_test_wait(&bars->kv_full[t % NS], (t / NS) & 1) &&
+          if (j < nk[i] && mbar_test_wait(&bars->kv_full[j % NS], (j / NS) & 1) &&
               (Cfg::kAliasP ? jp[i] >= j - 1  // PV(j - 2), which reads P there, is issued
                             : j == 0 || mbar_test_wait(&bars->s_free[i], (j - 1) & 1))) {
             tc::fence_after_sync();
-            issue_s(i, t % NS, place);
+            issue_s(i, j % NS, place);
             tc::commit(&bars->s_full[i][place]);
             js[i] = j + 1;
             did = true;
           }
           const int jq = jp[i];
           if (jq < js[i] && mbar_test_wait(&bars->p_full[i], jq & 1)) {
-            const int tq = stride * jq + odd * i;
             tc::fence_after_sync();
-            issue_pv(i, tq % NS, Cfg::kAliasP ? jq & 1 : 0, jq > 0);
+            issue_pv(i, jq % NS, Cfg::kAliasP ? jq & 1 : 0, jq > 0);
             tc::commit(&bars->pv_done[i]);
             jp[i] = jq + 1;
             did = true;
             // a stage is free once every stream that reads it has issued its PV
-            if (halves || jp[1 - i] > jq || jq >= nk[1 - i]) tc::commit(&bars->kv_empty[tq % NS]);
+            if (jp[1 - i] > jq || jq >= nk[1 - i]) tc::commit(&bars->kv_empty[jq % NS]);
           }
         }
         if (did) {
@@ -335,7 +326,7 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars->s_free[i]);
         }
-        const int keys = (it.end - it.begin) * kBS - (stride * j + odd * i) * BN;  // of this tile
+        const int keys = (it.end - it.begin) * kBS - j * BN;  // of this tile
         if (keys < BN) {
 #pragma unroll
           for (int c = 0; c < BN; ++c) x[c] = c < keys ? x[c] : -INFINITY;
@@ -359,7 +350,7 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
         }
         const float neg_m = m == -INFINITY ? 0.f : -m;
         // a warp waits only for a hand-off that its partner will make
-        if (partner && (i == 0 ? (j >= 1 && j - 1 < n1) : j < n0)) {
+        if (partner && (i == 1 || j > 0)) {
           const bool mine = !stopped(abort_flag) &&
                             mbar_wait(&bars->turn[i][quad], (i == 0 ? j - 1 : j) & 1, a.status,
                                       a.wait_limit);
@@ -419,8 +410,8 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
           ok && n > 0 && __all_sync(0xffffffffu, mbar_wait(&bars->pv_done[i], (n - 1) & 1,
                                                            a.status, a.wait_limit));
       if (ok && n > 0 && !done) *abort_flag = 1;
-      const int rr = it.row0 + (halves ? 0 : 128 * i) + r;
-      const int part = it.part + i * it.step + rr / group;
+      const int rr = it.row0 + 128 * i + r;
+      const int part = it.part + rr / group;
       const size_t at = size_t(part) * a.H + g * group + rr % group;
       if (done) {
         tc::fence_after_sync();

@@ -172,6 +172,8 @@ class B200Engine:
 
     # ------------------------------------------------------------------ submission
     def submit(self, request) -> None:
+        if self.per_request_sampling:
+            self._request_sampling(request)  # bad settings raise here, not in a later step
         self._incoming.append(request)
 
     def submit_many(self, requests) -> None:
@@ -225,11 +227,15 @@ class B200Engine:
         self._uniform.forget(req.request_id)
 
     # ------------------------------------------------------------------ sampling
+    @staticmethod
+    def _request_sampling(request) -> SamplingParams:
+        return SamplingParams(request.temperature, request.top_k, request.top_p,
+                              getattr(request, "min_p", 0.0))
+
     def _draws(self, batch: List, ahead: int = 0) -> tuple:
         """(settings, numbers) for each request's next token, or the one `ahead` after."""
         if self.per_request_sampling:
-            params = [SamplingParams(r.temperature, r.top_k, r.top_p, getattr(r, "min_p", 0.0))
-                      for r in batch]
+            params = [self._request_sampling(r) for r in batch]
         else:
             params = [self.sampling] * len(batch)
         return params, self._uniform([r.request_id for r in batch],

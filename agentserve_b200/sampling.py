@@ -39,8 +39,6 @@ class SamplingParams:
         return not self.temperature > 1e-6
 
 
-GREEDY = SamplingParams(temperature=0.0)
-
 # rows of the int32 staging buffer after the decode step's own (tokens, lengths, table rows)
 STAGED = 5
 

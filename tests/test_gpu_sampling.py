@@ -7,6 +7,10 @@ Log-probabilities: fp32 rounding of the result (2^-24 relative) and of nothing e
 64-bit values behind both sides agree to 1e-11, so rtol is 2^-24 + 1e-11 and the
 absolute part 1e-11."""
 
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -191,6 +195,24 @@ def test_sample_rows_from_every_alignment(B, V, dtype):
                            x.float().argmax(1))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_sample_row_does_not_depend_on_its_batch(dtype):
+    """Rows in batches of every cluster size: the sums are exact, so tokens and
+    log-probabilities are the same bits."""
+    x = random_logits(160, 70001, 5, dtype)
+    g = torch.Generator(device=DEV).manual_seed(9)
+    u = torch.rand(160, generator=g, device=DEV)
+    T = 0.3 + torch.rand(160, generator=g, device=DEV)
+    k = torch.randint(0, 400, (160,), generator=g, device=DEV, dtype=torch.int32)
+    p = 0.7 + 0.4 * torch.rand(160, generator=g, device=DEV)
+    want_lp = torch.empty(160, device=DEV)
+    want = ops.sample_tokens(x, u, T, k, p, logprobs=want_lp)
+    for n in (1, 7, 16, 17, 33, 34, 36, 71, 72, 75, 148, 149):
+        lp = torch.empty(n, device=DEV)
+        tok = ops.sample_tokens(x[:n], u[:n], T[:n], k[:n], p[:n], logprobs=lp)
+        assert torch.equal(tok, want[:n]) and torch.equal(lp, want_lp[:n]), n
+
+
 def test_sample_frequencies_follow_the_probabilities():
     """Equally spaced u over one row give every kept token its share: the number of the
     N values that fall in a token's interval is off by less than one at either end."""
@@ -228,3 +250,24 @@ def test_sample_is_the_same_in_a_graph_and_on_another_stream():
         u.copy_(torch.rand(16, generator=torch.Generator().manual_seed(seed)))
         graph.replay()
         assert torch.equal(out, ops.sample_tokens(x, u, T, k, p))
+
+
+def test_sample_first_call_of_a_process_is_captured():
+    """Nothing that the library sets up on a first call breaks a capture."""
+    code = """
+import torch
+from agentserve_b200 import ops
+x = torch.randn(20, 50001, device='cuda').half()
+u, T = torch.rand(20, device='cuda'), torch.full((20,), 0.9, device='cuda')
+out = torch.empty(20, dtype=torch.int64, device='cuda')
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    ops.sample_tokens(x, u, T, out=out)
+graph.replay()
+assert torch.equal(out, ops.sample_tokens(x, u, T))
+"""
+    root = Path(__file__).resolve().parents[1]
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
+                         timeout=300)
+    assert run.returncode == 0, run.stderr

@@ -7,8 +7,10 @@ import random
 import numpy as np
 import pytest
 
-from agentserve_b200 import B200Engine, DeviceBlockAllocator, SamplingParams, UniformStream
+from agentserve_b200 import (B200Engine, DeviceBlockAllocator, Request, SamplingParams,
+                             UniformStream)
 from agentserve_b200 import sampling as S
+from tests.test_engine_host import FAKE_CFG, E
 
 
 def test_settings_are_checked():
@@ -59,6 +61,23 @@ def test_engine_refuses_sampling_without_a_sampling_model():
         B200Engine(None, model=Greedy(), temperature=0.8, top_p=0.0)
     with pytest.raises(ValueError, match="shared-prefix"):
         B200Engine(None, model=Greedy(), shared_prefix_attention=True)
+
+
+def test_bad_settings_of_a_request_raise_when_it_is_submitted():
+    """Not in a later step, which other requests share."""
+    class Sampled(E.HistoryModelForB200):
+        def prefill_paged_sampled(self, *args):
+            raise AssertionError("no step runs here")
+
+    engine = B200Engine(FAKE_CFG, model=Sampled(), num_cache_blocks=64, per_request_sampling=True)
+    good = Request(prompt="a", token_ids=[1, 2], max_tokens=2, temperature=0.7, top_p=0.9)
+    bad = Request(prompt="b", token_ids=[1, 2], max_tokens=2, temperature=0.7, top_p=0.0)
+    engine.submit(good)
+    with pytest.raises(ValueError, match="top_p"):
+        engine.submit(bad)
+    with pytest.raises(ValueError, match="top_p"):
+        engine.submit_many([bad])
+    assert list(engine._incoming) == [good]
 
 
 def allocator(lists):

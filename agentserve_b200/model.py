@@ -195,10 +195,10 @@ class B200LlamaModel(nn.Module):
         self.shared_prefix_decode: bool = False
         # Block reads (members - 1 times shared blocks, over all groups) that sharing must
         # save: below, the per-request launch is faster.  B200, rotation included, per
-        # layer, fused against shared: 16 sequences on 64 blocks (960 saved) 12.8 / 17.4 us
-        # at head_dim 64 and 19.0 / 20.9 at 128; on 128 (1,920) 18.4 / 18.1 and 31.8 /
-        # 22.3; 64 on 32 (2,016) 22.9 / 23.3 and 40.7 / 29.6; 64 on 256 61.0 / 29.2 and
-        # 112 / 38.8.
+        # layer, fused against shared: 16 sequences on 64 blocks (960 saved) 12.7 / 16.7 us
+        # at head_dim 64 and 18.8 / 20.2 at 128; on 128 (1,920) 18.3 / 18.4 and 31.9 /
+        # 22.9; 64 on 32 (2,016) 22.8 / 23.0 and 40.2 / 28.7; 64 on 256 61.4 / 28.8 and
+        # 113 / 36.8.
         self.shared_prefix_min_saved: int = 1920
         self._prefix_groups: Optional[tuple] = None  # (allocator, its epoch, requests, groups)
         self.max_decode_graphs: int = 16

@@ -414,18 +414,42 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
       const int part = it.part + rr / group;
       const size_t at = size_t(part) * a.H + g * group + rr % group;
       if (done) {
+        // A row per thread in TMEM.  Of many rows, O goes by way of this warp's part of Q,
+        // which no MMA of the stream reads any more, to global memory in whole lines: 64
+        // sequences (256 rows) on 4,096 tokens 19.8 us, straight from the threads 20.6.  Of
+        // few rows straight: 4 (16 rows) on 160 8.1 us, by way of Q 8.6; 16 (64 rows) on
+        // 8,000 17.4 and 17.8; 32 (128 rows) on 14,336 22.6 and 22.2.
+        const bool lines = it.rows > 64;
         tc::fence_after_sync();
+        uint8_t* mine = smem + i * Cfg::kQBytes + quad * 4096;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           tc::ld_32x32b_x32(tO + c * 32, o);
           tc::wait_ld();
-          if (r < my_rows) {
-            uint4* dst = reinterpret_cast<uint4*>(a.parts.o + at * D + c * 32);
+          if (!lines) {
+            if (r < my_rows) {
+              uint4* dst = reinterpret_cast<uint4*>(a.parts.o + at * D + c * 32);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+              for (int e = 0; e < 8; ++e)
+                dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            }
+            continue;
           }
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<uint4*>(mine + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+                make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int row = 4 * k + (lane >> 3), e = lane & 7;
+            const size_t to = __shfl_sync(0xffffffffu, static_cast<unsigned long long>(at), row);
+            if (quad * 32 + row < my_rows)
+              *reinterpret_cast<uint4*>(a.parts.o + to * D + c * 32 + e * 4) =
+                  *reinterpret_cast<const uint4*>(mine + row * 128 + ((e ^ (row & 7)) << 4));
+          }
+          __syncwarp();
         }
       }
       if (r < my_rows) a.parts.ml[at] = done ? make_float2(m, l) : make_float2(-INFINITY, 0.f);

@@ -19,6 +19,10 @@
 // total: weights are computed in 64 bits and summed in fixed point (units of 2^-42 of
 // the largest), which makes every sum exact and independent of the order of the atomics.
 //
+// Few rows are bound by latency (a cluster barrier or a pass of few tokens costs about 1K
+// cycles: one bf16 row of 128,256 tokens, top-p, 19 us, of which the logits' bytes are 0.04),
+// many by integer instructions and shared-memory atomics (256 rows 83 us, 66 MB read twice).
+//
 // A row is worked on by a cluster of 1 to 8 CTAs, each holding a run of indexes, its warps
 // runs of that; they exchange totals over distributed shared memory.  Every decision
 // follows from exchanged values, so all CTAs of a cluster take the same barriers.

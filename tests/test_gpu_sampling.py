@@ -252,6 +252,29 @@ def test_sample_is_the_same_in_a_graph_and_on_another_stream():
         assert torch.equal(out, ops.sample_tokens(x, u, T, k, p))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("value", [0.0, 1.0, -3.0])
+def test_sample_the_largest_vocabulary_of_equal_tokens(dtype, value):
+    """2^20 tokens of weight 1, the largest sums there are: u picks index u V of the V kept
+    ones (exactly, V a power of two), the first V p of them under top-p."""
+    V = 1 << 20
+    u = [0.0, 0.25, 0.5 + 2.0 ** -20, 0.7109375, 1.0 - 2.0 ** -20]
+    flat = torch.full((3 + len(u) * (V + 1),), 50.0, dtype=dtype, device=DEV)
+    x = flat[3:].view(len(u), V + 1)[:, :V]
+    x.fill_(value)
+    ones = [1.0] * len(u)
+    for p, kept in ((1.0, V), (0.5, V // 2), (0.0625, V // 16)):
+        lp = torch.empty(len(u), device=DEV)
+        tok = ops.sample_tokens(x, rows_of(u, torch.float32), rows_of(ones, torch.float32), None,
+                                rows_of([p] * len(u), torch.float32), logprobs=lp)
+        assert tok.tolist() == [int(v * kept) for v in u]
+        torch.testing.assert_close(lp, torch.full_like(lp, -float(np.log(kept))),
+                                   rtol=2.0 ** -24 + 1e-11, atol=0)
+    k = rows_of([1000, 1, V, V - 1, 3], torch.int32)
+    tok = ops.sample_tokens(x, rows_of(u, torch.float32), rows_of(ones, torch.float32), k)
+    assert tok.tolist() == [int(v * n) for v, n in zip(u, k.tolist())]
+
+
 def test_sample_first_call_of_a_process_is_captured():
     """Nothing that the library sets up on a first call breaks a capture."""
     code = """

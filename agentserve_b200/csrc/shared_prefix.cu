@@ -75,6 +75,10 @@ sp_generic_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
     row0 = it.row0 + blockIdx.z * Cfg::kRows;  // the plan's tiles may be larger
     rows = min(Cfg::kRows, it.rows - int(blockIdx.z) * Cfg::kRows);
     if (rows <= 0) return;
+    if (it.end > a.max_blocks) {  // of a group that row_plan() attends alone: not in the table
+      if (threadIdx.x == 0) flag_status(a.status, kStatusBadLength);
+      return;
+    }
     begin = it.begin * kBS;
     end = it.end * kBS;
     part = it.part;

@@ -82,7 +82,9 @@ __device__ __forceinline__ Item load_item(const Item* items, int i) {
 }
 
 // A row's own keys and what of its shared part counts.  A row shorter than its group's
-// shared part takes nothing from it: all its keys are its own.
+// shared part takes nothing from it: all its keys are its own.  So does every row of a group
+// that shares more blocks than the table holds (a captured launch, whose plan was replaced):
+// rows are cut to the table.
 struct RowPlan {
   int shared, prefix_splits, prefix_part, prefix_step, own_splits, own_part;
   int len, begin, count;  // keys; this item's blocks

@@ -99,6 +99,10 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
   pdl_trigger();  // every block of this launch has started: the own launch may start
   const PrefixItem it = load_item(a.prefix_items, blockIdx.x);
   if (it.rows == 0) return;
+  if (it.end > a.max_blocks) {  // of a group that row_plan() attends alone: not in the table
+    if (threadIdx.x == 0) flag_status(a.status, kStatusBadLength);
+    return;
+  }
   const int g = blockIdx.y, group = a.group;
   const int n_tiles = (it.end - it.begin + NB - 1) / NB;
   // streams: rows and key tiles of each

@@ -333,7 +333,9 @@ class SharedPrefixPlan:
     def load(self, groups: Sequence[Sequence[int]], prefix_blocks: Sequence[int],
              row_blocks: Sequence[int]) -> None:
         """Replace the plan by another of the same batch size, in the same buffers; with
-        full_grid, launches captured with this plan follow it.  Stream-ordered."""
+        full_grid, launches captured with this plan follow it.  Stream-ordered.  A group that
+        shares more blocks than a captured launch's table holds is attended row by row there,
+        and sets device status bit 16."""
         _require(len(groups) == len(prefix_blocks) and len(row_blocks) == self.num_seqs,
                  "shared_prefix_plan: one prefix_blocks per group and one row_blocks per sequence")
         offsets = np.zeros(len(groups) + 1, dtype=np.int32)

@@ -255,7 +255,9 @@ AS_API int as_paged_decode_attention_noalloc(void* out, const void* q, int64_t q
  * device copy, and the host copy's first AS_SHARED_PREFIX_HEADER ints, which size the
  * launch.  full_grid != 0 sizes it for any plan of the same batch size and geometry,
  * so that a captured launch may be replayed after another plan was copied over the
- * device buffer; 0 sizes it for this plan.  A plan with no group is valid.
+ * device buffer; 0 sizes it for this plan.  A plan with no group is valid.  A plan that
+ * shares more blocks than the table holds (max_blocks) is refused; in a replay, where that
+ * is found on the device, it sets status bit 16 and the group's rows are attended alone.
  *
  * The attention itself: seq_lens_k counts the new token, whose K/V must be in the pool.
  * A row shorter than its group's shared blocks is attended alone (correct, not shared);

@@ -98,7 +98,7 @@ __device__ __forceinline__ RowPlan row_plan(const Args& a, const OwnItem& it, bo
   p.own_splits = it.own_splits;
   p.own_part = a.own_part0 + it.own_part;
   p.len = max(0, a.seq_lens[it.row]);
-  int blocks = (p.len + kBS - 1) / kBS;
+  int blocks = p.len / kBS + (p.len % kBS != 0);  // any length: no sum past 31 bits
   if (blocks > a.max_blocks) {
     if (flag) flag_status(a.status, kStatusBadLength);
     blocks = a.max_blocks;

@@ -44,3 +44,22 @@ def test_a_replayed_plan_wider_than_its_table_is_flagged_and_right(dtype, D):
     out.zero_()
     graph.replay()
     b.check(out)
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (HF, 128), (FP, 64)])
+@pytest.mark.parametrize("n", [2 ** 31 - 1, 2 ** 31 - 15, 2 ** 31 - 17, 1 << 30])
+def test_lengths_near_the_end_of_32_bits_are_flagged_and_cut(dtype, D, n):
+    """A row's length past its table: the row is cut to the table, whatever the length."""
+    b = Batch(8, 2, D, dtype, [800, 790, 795, 790], [([0, 1], 30)], seed=32)
+    wide = torch.full((4, 300), 1 << 30, dtype=torch.int32, device=DEV)
+    wide[:, :50] = b.table[:, :50]
+    b.table = wide[:, :50]
+    want = b.run()
+    b.check(want)
+    b.lens[0] = b.lens[2] = 800  # the whole table
+    b.table[2, 49] = b.table[1, 49]
+    want = b.run().clone()
+    assert ops.device_status(clear=True) == 0
+    b.lens[0] = b.lens[2] = n
+    assert torch.equal(b.run(), want)
+    assert ops.device_status(clear=True) == 16

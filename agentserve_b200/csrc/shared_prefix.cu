@@ -253,6 +253,9 @@ constexpr int64_t kOwnOverhead = 16;
 // Least own blocks of an item, where a row has that many: with 4, 16 fp32 sequences on 1,024
 // take 34 us instead of 27; with 16 as with 8.
 constexpr int64_t kMinOwn = 8;
+// Most blocks of a row: its keys are counted in 31 bits.
+constexpr int kMostBlocks = (1 << 27) - 1;
+static_assert(int64_t(kMostBlocks) * kBS < int64_t(1) << 31, "keys");
 
 template <typename T, int DP, int RW, int TG, bool kPrefix>
 int launch_generic_one(dim3 grid, int tile_rows, T* out, const T* q, const T* k, const T* v, const Args& a,
@@ -412,6 +415,11 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
     std::vector<int> list;
     if (num_groups && group_offsets[0] != 0)
       return fail(AS_ERR_INVALID_ARG, "%s: group_offsets must start at 0", who);
+    for (int b = 0; b < B; ++b) {
+      if (row_blocks[b] < 0) return fail(AS_ERR_INVALID_ARG, "%s: negative row_blocks", who);
+      if (row_blocks[b] > kMostBlocks)  // bounds the shared blocks too, checked below
+        return fail(AS_ERR_INVALID_ARG, "%s: row_blocks past %d", who, kMostBlocks);
+    }
     for (int i = 0; i < num_groups; ++i) {
       const int lo = group_offsets[i], hi = group_offsets[i + 1];
       if (lo > hi || hi > B)
@@ -439,8 +447,6 @@ extern "C" int as_shared_prefix_plan(int32_t* plan, int64_t capacity,
       }
       groups.push_back(g);
     }
-    for (int b = 0; b < B; ++b)
-      if (row_blocks[b] < 0) return fail(AS_ERR_INVALID_ARG, "%s: negative row_blocks", who);
 
     // prefix splits: pieces of about equal length, in units of 8 blocks (half units on
     // tensor cores, for the fixed cost)

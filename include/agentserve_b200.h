@@ -248,9 +248,9 @@ AS_API int as_paged_decode_attention_noalloc(void* out, const void* q, int64_t q
  * batch rows members[group_offsets[i] .. group_offsets[i+1]-1] whose block tables start
  * with the same prefix_blocks[i] blocks; no row may be in two groups, and rows in none
  * attend alone.  row_blocks[b] is the number of blocks row b will hold (at least its
- * group's prefix_blocks; used to balance the work, the lengths themselves are read on
- * the device at every call).  The plan stays valid while the same rows share the same
- * blocks.  plan: as_shared_prefix_plan_ints() ints of host memory (`capacity` of them
+ * group's prefix_blocks, less than 2^27; used to balance the work, the lengths themselves
+ * are read on the device at every call).  The plan stays valid while the same rows share
+ * the same blocks.  plan: as_shared_prefix_plan_ints() ints of host memory (`capacity` of them
  * available).  The caller copies all of them to the device, and passes both: the
  * device copy, and the host copy's first AS_SHARED_PREFIX_HEADER ints, which size the
  * launch.  full_grid != 0 sizes it for any plan of the same batch size and geometry,

@@ -153,8 +153,8 @@ __device__ void finish_own(const Args& a, const RowPlan& p, T* __restrict__ out,
 #pragma unroll
       for (int w = 0; w < kSub; ++w) {
         const float x = m[w * kRows + r];
-        if (x == -INFINITY) continue;
-        const float e = part_exp<kBase2>(x - M);
+        // no keys (l = o = 0), or NaN in all of them, which the sums keep
+        const float e = x == -INFINITY ? 0.f : part_exp<kBase2>(x - M);
         L += e * l[w * kRows + r];
         O += e * o[(w * kRows + r) * ld + d];
       }

@@ -134,7 +134,7 @@ struct alignas(16) Shared {
   Slot slot[2][kMaxCluster];  // exchanges, in turn
   Slot found, found2;
   u64 warp[kWarps];
-  int flag;
+  uint32_t flag;
   uint32_t n_list;     // tokens left in this CTA's run; the first of them
   float list[kList];
   float left[kList];   // the cluster's, and what each measures
@@ -153,7 +153,7 @@ static_assert(sizeof(Queue) >= 3 * kBins * 4 && kThreads == kBins / 2, "find() s
 // nothing next to any maximum this path accepts.  The first pass then needs no maximum
 // and no exponential, both cuts come from one merge, and the second pass looks the
 // weights up.  Rows outside this (values of 128 and more, NaN, cuts among the listed
-// values, u <= 0) take the general path.
+// values, u <= 0 or >= 1) take the general path.
 //
 // 64 rows of 128,256 tokens, top-p: 34 us, and 83 by the general path (fp16).  The passes
 // are bound by integer instructions (half rate), so a value's place is two
@@ -886,6 +886,37 @@ __device__ __noinline__ Cuts value_cuts(Row<__nv_bfloat16> w, ByValue& bv, int k
   return r;
 }
 
+// The row's token for a u outside (0, 1): the first or last kept one whose weight is positive
+// in 64 bits (above 2^-1074).  Of the tokens at the cut those are kept before which there are
+// fewer than `ties` in index order; `seen` of them come before this warp's run.  s.flag is 0.
+template <typename T>
+__device__ __noinline__ int end_of_kept(Row<T> w, float cut, u64 ties, u64 seen, bool last) {
+  constexpr int VEC = Row<T>::VEC;
+  uint32_t best = 0;  // ~index or index + 1: the largest is wanted
+  w.visit([&](const float(&x)[VEC], int i) {
+    uint32_t n = 0;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) n += x[j] == cut;
+    const u64 upto = seen + warp_scan(n);  // with this lane's own
+    u64 at = upto - n;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const bool kept = x[j] > cut || (x[j] == cut && at < ties);
+      at += x[j] == cut;
+      if (kept && (double(x[j]) - w.md) * w.c > -1074.0)
+        best = max(best, last ? uint32_t(i + j) + 1 : ~uint32_t(i + j));
+    }
+    seen = __shfl_sync(0xffffffffu, upto, 31);
+  });
+  best = __reduce_max_sync(0xffffffffu, best);
+  if ((threadIdx.x & 31) == 0) atomicMax(&w.sp->flag, best);
+  __syncthreads();
+  const Slot* all = w.exchange(Slot{w.sp->flag, 0, 0});
+  best = 0;  // the maximum is kept: some warp has one
+  for (int q = 0; q < w.C; ++q) best = max(best, uint32_t(all[q].a));
+  return int(last ? best - 1 : ~best);
+}
+
 // The least value whose weight is at least min_p, by steps from its closed form.
 __device__ __noinline__ float least_kept(float m, double T, double min_p) {
   const double at = double(m) + T * log(min_p);
@@ -984,7 +1015,7 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
            __reduce_max_sync(0xffffffffu, uint32_t(v));
   };
   mine.a = block_max(ord_key(mx), special != 0);
-  if (kByValue && (bv.refuse || !(u > 0.f))) mine.a |= 1ull << 32;
+  if (kByValue && (bv.refuse || !(u > 0.f && u < 1.f))) mine.a |= 1ull << 32;
   cluster_wait_started(p.C);
   const Slot* all = w.exchange(mine);
   uint32_t top = 0;
@@ -1119,17 +1150,8 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
     kept = sum_above(w, cut, false);
   const Scan ws = block_scan(s, lane == 0 ? kept.sum : 0);
   const Scan wt = block_scan(s, lane == 0 ? kept.ties : 0);
-  uint32_t low = 0xffffffffu;
-  if (!(u > 0.f)) {  // the first kept token of positive weight (in 64 bits: above 2^-1074)
-    w.visit([&](const float(&x)[VEC], int i) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        if (x[j] >= cut && (double(x[j]) - w.md) * w.c > -1074.0) low = min(low, uint32_t(i + j));
-    });
-    low = ~uint32_t(block_max(~low, 0));
-  }
-  all = w.exchange(Slot{ws.total, wt.total, (u64(__float_as_uint(u)) << 32) | low});
-  const float uu = __uint_as_float(uint32_t(all[0].c >> 32));
+  all = w.exchange(Slot{ws.total, wt.total, __float_as_uint(u)});
+  const float uu = __uint_as_float(uint32_t(all[0].c));
   const u64 wcut = cut == -INFINITY ? 0 : w.weight(cut);
   u64 before = 0, total = 0, t_before = 0, t_all = 0;
   for (int q = 0; q < p.C; ++q) {
@@ -1139,7 +1161,6 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
     }
     total += all[q].a;
     t_all += all[q].b;
-    low = min(low, uint32_t(all[q].c));
   }
   total += min(ties, t_all) * wcut;
   // lane 0's: what comes before this warp's run, and what the run holds
@@ -1153,13 +1174,13 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
       p.logprobs[r] =
           float((double(x) - double(m)) / T64 - log(double(total) / double(1ull << kFrac)));
   };
-  if (!(uu > 0.f)) {
-    if (w.rank == 0 && t == 0 && low < uint32_t(p.V))
-      write(int(low), sanitize(Elem<T>::to_f32(w.row[low])));
+  if (!(uu > 0.f && uu < 1.f)) {
+    const u64 seen = __shfl_sync(0xffffffffu, t_before, 0);
+    const int i = end_of_kept(w, cut, ties, seen, uu >= 1.f);
+    if (w.rank == 0 && t == 0) write(i, sanitize(Elem<T>::to_f32(w.row[i])));
     return;
   }
-  u64 target = u64(double(uu) * double(total));
-  if (target >= total) target = total - 1;
+  const u64 target = u64(double(uu) * double(total));  // u < 1: below the total
   const auto weight = [&](float x) -> u64 {  // of a token above the cut
     if constexpr (kByValue) {
       const uint32_t code = __float_as_uint(x) >> 16;
@@ -1267,7 +1288,7 @@ struct SmallShared {
   u64 weight[kSmall];  // by index
   u64 z;
   int n;
-  uint32_t low;
+  uint32_t low, high;  // first and last kept index of positive weight
 };
 
 static_assert(sizeof(SmallShared) + 1024 <= 64 * 1024, "shared memory");
@@ -1291,7 +1312,10 @@ sample_small_kernel(const T* __restrict__ logits, const Params p) {
     sm.key[i] = i < V ? (u64(ord_key(sanitize(Elem<T>::to_f32(row[i])))) << 32) | ~uint32_t(i) : 0;
     sm.weight[i] = 0;
   }
-  if (t == 0) sm.low = 0xffffffffu;
+  if (t == 0) {
+    sm.low = 0xffffffffu;
+    sm.high = 0;
+  }
   __syncthreads();
 #pragma unroll 1
   for (int size = 2; size <= N; size *= 2) {
@@ -1351,7 +1375,10 @@ sample_small_kernel(const T* __restrict__ logits, const Params p) {
     const int i = t * per + e;
     if (i >= n) break;
     sm.weight[index(i)] = w[e];
-    if (positive >> e & 1) atomicMin(&sm.low, uint32_t(index(i)));
+    if (positive >> e & 1) {
+      atomicMin(&sm.low, uint32_t(index(i)));
+      atomicMax(&sm.high, uint32_t(index(i)));
+    }
   }
   __syncthreads();
   sum = 0;
@@ -1363,12 +1390,11 @@ sample_small_kernel(const T* __restrict__ logits, const Params p) {
     if (p.logprobs)
       p.logprobs[r] = float((double(x) - double(m)) / T64 - log(double(is.total) / one));
   };
-  if (!(u > 0.f)) {
-    if (t == 0) write(int(sm.low));
+  if (!(u > 0.f && u < 1.f)) {
+    if (t == 0) write(int(u >= 1.f ? sm.high : sm.low));
     return;
   }
-  u64 target = u64(double(u) * double(is.total));
-  if (target >= is.total) target = is.total - 1;
+  const u64 target = u64(double(u) * double(is.total));  // u < 1: below the total
   if (!(is.before <= target && target < is.before + sum)) return;
   u64 run = is.before;
   for (int i = t * per; i < V; ++i) {

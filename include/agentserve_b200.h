@@ -390,8 +390,10 @@ AS_API int as_greedy_argmax(int64_t* out, const void* logits, int64_t row_stride
  * the first maximum, as as_greedy_argmax.  logprobs[r] (NULL to skip) is the log of the
  * token's weight over the kept total, 0 for a row that keeps one token.
  * u, temperature, top_p, min_p fp32 and top_k int32 are [num_rows]; top_k, top_p and
- * min_p may be NULL (off).  Weights are computed in 64 bits and summed in fixed point,
- * so the result does not depend on the launch; no workspace.  vocab <= 2^20. */
+ * min_p may be NULL (off).  Weights are computed in 64 bits and summed in units of 2^-42 of
+ * the row's largest weight, so the result does not depend on the launch; a token below
+ * 2^-43 of the largest adds nothing to a sum, and no u inside (0, 1) draws it.  No
+ * workspace.  vocab <= 2^20. */
 AS_API int as_sample_tokens(int64_t* out, float* logprobs, const void* logits,
                             int64_t row_stride, const float* u, const float* temperature,
                             const int32_t* top_k, const float* top_p, const float* min_p,

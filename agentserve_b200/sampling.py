@@ -33,11 +33,17 @@ class SamplingParams:
             raise ValueError(f"top_p must be in (0, 1], got {self.top_p}")
         if not 0.0 <= self.min_p <= 1.0:
             raise ValueError(f"min_p must be in [0, 1], got {self.min_p}")
+        try:
+            int(self.top_k)
+        except (TypeError, ValueError, OverflowError):
+            raise ValueError(f"top_k must be a whole number, got {self.top_k!r}") from None
 
     @property
     def greedy(self) -> bool:
         return not self.temperature > 1e-6
 
+
+_GREEDY = SamplingParams(temperature=0.0)
 
 # rows of the int32 staging buffer after the decode step's own (tokens, lengths, table rows)
 STAGED = 5
@@ -45,12 +51,14 @@ STAGED = 5
 
 def stage(out: np.ndarray, params: Sequence[SamplingParams], u: Sequence[float]) -> None:
     """Writes a batch's settings and numbers into out [5, B] int32: temperature, top_k,
-    top_p, min_p and u, the fp32 ones by their bits; rows past the batch are greedy."""
+    top_p, min_p and u, the fp32 ones by their bits; rows past the batch are greedy.  Nothing
+    else of a greedy request is read."""
     n = len(params)
+    params = [_GREEDY if p.greedy else p for p in params]
     f = out.view(np.float32)
     out[:] = 0
     f[0, :n] = [p.temperature for p in params]
-    out[1, :n] = [min(max(p.top_k, 0), 2 ** 31 - 1) for p in params]
+    out[1, :n] = [min(max(int(p.top_k), 0), 2 ** 31 - 1) for p in params]
     f[2] = 1.0
     f[2, :n] = [p.top_p for p in params]
     f[3, :n] = [p.min_p for p in params]

@@ -26,6 +26,7 @@ keeps the new token's K/V.
 from __future__ import annotations
 
 import math
+import weakref
 from collections import OrderedDict
 from typing import List, Optional, Sequence
 
@@ -200,7 +201,8 @@ class B200LlamaModel(nn.Module):
         # 22.9; 64 on 32 (2,016) 22.8 / 23.0 and 40.2 / 28.7; 64 on 256 61.4 / 28.8 and
         # 113 / 36.8.
         self.shared_prefix_min_saved: int = 1920
-        self._prefix_groups: Optional[tuple] = None  # (allocator, its epoch, requests, groups)
+        # (weak reference to the allocator, its epoch, requests, groups, shared blocks)
+        self._prefix_groups: Optional[tuple] = None
         self.max_decode_graphs: int = 16
         self._graphs: "OrderedDict[tuple, _PagedStepGraph]" = OrderedDict()
         self._graph_pool = None
@@ -649,12 +651,13 @@ class B200LlamaModel(nn.Module):
             return None
         known = self._prefix_groups
         rids = tuple(request_ids)
-        if not (known is not None and known[0] is allocator and known[1] == allocator.epoch
+        if not (known is not None and known[0]() is allocator and known[1] == allocator.epoch
                 and known[2] == rids):
             groups, blocks = allocator.shared_prefix_groups(rids)
             if sum((len(g) - 1) * n for g, n in zip(groups, blocks)) < self.shared_prefix_min_saved:
                 groups, blocks = [], []
-            known = self._prefix_groups = (allocator, allocator.epoch, rids, groups, blocks)
+            known = self._prefix_groups = (weakref.ref(allocator), allocator.epoch, rids, groups,
+                                           blocks)
         if not known[3]:
             return None
         rows = [len(allocator._request_blocks[r]) for r in rids]
@@ -787,6 +790,7 @@ class B200LlamaModel(nn.Module):
             g.release()
         self._graphs.clear()
         self._graph_pool = None
+        self._prefix_groups = None
         if self._batch_pool is not None and self._batch_pool.get("graph") is not None:
             self._batch_pool.pop("graph").reset()  # forward_decode_batch's captured step
 

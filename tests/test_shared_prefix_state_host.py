@@ -1,0 +1,46 @@
+"""What the model keeps of a batch's shared blocks between steps (host code)."""
+
+import gc
+import weakref
+
+import pytest
+import torch
+
+from agentserve_b200 import B200LlamaModel, DeviceBlockAllocator, ModelConfig
+
+CFG = ModelConfig(hidden_dim=128, n_heads=2, n_kv_heads=1, n_layers=1, vocab_size=50,
+                  max_seq_len=512, intermediate_size=64)
+
+
+def make_model():
+    model = B200LlamaModel(CFG, dtype=torch.float32, device="cpu")
+    model.shared_prefix_decode = True
+    return model
+
+
+def make_allocator(shared=10, requests=("a", "b", "c")):
+    alloc = DeviceBlockAllocator(100, device="cpu", allocate_tensor=False, max_seqs=8,
+                                 max_blocks_per_seq=64)
+    ids = alloc.allocate(requests[0], shared + 2)
+    for r in requests[1:]:
+        alloc.share_blocks(r, ids[:shared])
+        alloc.allocate(r, 2)
+    return alloc
+
+
+def test_a_dropped_allocator_is_released(monkeypatch):
+    """The groups of the last batch keep neither the pool nor, past release_decode_graphs(),
+    anything of it."""
+    model, alloc = make_model(), make_allocator()
+    model.shared_prefix_min_saved = 1
+    assert model._sharing(alloc, ["a", "b", "c"]) == ([[0, 1, 2]], [10], [12] * 3)
+    gone = weakref.ref(alloc)
+    del alloc
+    gc.collect()
+    assert gone() is None
+    other = make_allocator(shared=6)  # of the same epoch and requests
+    assert model._sharing(other, ["a", "b", "c"]) == ([[0, 1, 2]], [6], [8] * 3)
+    assert model._prefix_groups is not None
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda: None)
+    model.release_decode_graphs()
+    assert model._prefix_groups is None

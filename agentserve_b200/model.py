@@ -654,11 +654,10 @@ class B200LlamaModel(nn.Module):
         if not (known is not None and known[0]() is allocator and known[1] == allocator.epoch
                 and known[2] == rids):
             groups, blocks = allocator.shared_prefix_groups(rids)
-            if sum((len(g) - 1) * n for g, n in zip(groups, blocks)) < self.shared_prefix_min_saved:
-                groups, blocks = [], []
             known = self._prefix_groups = (weakref.ref(allocator), allocator.epoch, rids, groups,
                                            blocks)
-        if not known[3]:
+        saved = sum((len(g) - 1) * n for g, n in zip(known[3], known[4]))
+        if not saved or saved < self.shared_prefix_min_saved:
             return None
         rows = [len(allocator._request_blocks[r]) for r in rids]
         return known[3], known[4], rows + [1] * (batch - len(rows))

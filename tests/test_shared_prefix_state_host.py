@@ -44,3 +44,23 @@ def test_a_dropped_allocator_is_released(monkeypatch):
     monkeypatch.setattr(torch.cuda, "synchronize", lambda: None)
     model.release_decode_graphs()
     assert model._prefix_groups is None
+
+
+def test_the_threshold_holds_from_the_next_step(monkeypatch):
+    """shared_prefix_min_saved is read at every step, also while the groups are known."""
+    model, alloc = make_model(), make_allocator()
+    rids = ["a", "b", "c"]
+    assert model._sharing(alloc, rids) is None  # 20 block reads saved of 1,920
+    calls = []
+    find = alloc.shared_prefix_groups
+    monkeypatch.setattr(alloc, "shared_prefix_groups", lambda *a: calls.append(a) or find(*a))
+    for least, shares in ((20, True), (21, False), (0, True)):
+        model.shared_prefix_min_saved = least
+        assert (model._sharing(alloc, rids) is not None) == shares
+    assert not calls  # from the groups that were found before
+    alloc.free("c")
+    assert model._sharing(alloc, rids[:2]) == ([[0, 1]], [10], [12] * 2)
+    assert len(calls) == 1
+    alloc.free("b")
+    alloc.allocate("b", 3)
+    assert model._sharing(alloc, rids[:2]) is None  # nothing shared, whatever the threshold

@@ -48,6 +48,9 @@ class DeviceBlockAllocator:
         # hold until the next one)
         self.epoch = 0
         self._block_arrays: Dict[str, np.ndarray] = {}
+        # True: decode steps over this allocator read blocks that their requests share once
+        # per group of them, also where the model's own shared_prefix_decode is off
+        self.shared_prefix_decode = False
         # device block-table rows
         self.max_seqs = max_seqs
         self.max_blocks_per_seq = max_blocks_per_seq or num_blocks

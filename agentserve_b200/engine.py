@@ -127,10 +127,8 @@ class B200Engine:
         self.temperature, self.top_p, self.top_k = temperature, top_p, top_k
         self.model = model if model is not None else B200LlamaModel(config, dtype=dtype,
                                                                     device=device)
-        if shared_prefix_attention:
-            if not hasattr(self.model, "shared_prefix_decode"):
-                raise ValueError("the model has no shared-prefix decode attention")
-            self.model.shared_prefix_decode = True
+        if shared_prefix_attention and not hasattr(self.model, "shared_prefix_decode"):
+            raise ValueError("the model has no shared-prefix decode attention")
         self.device = self.model.device
         dtype = self.model.dtype
         # decode batches come in many (batch size, block bucket) shapes: keep their
@@ -152,6 +150,7 @@ class B200Engine:
             num_blocks=num_cache_blocks, block_size=block_size, num_layers=config.n_layers,
             num_kv_heads=self.model.Kh, head_dim=config.head_dim, dtype=dtype,
             device=self.device, max_seqs=max_seqs, max_blocks_per_seq=max_blocks_per_seq)
+        self.allocator.shared_prefix_decode = shared_prefix_attention
         self.prefix_cache = PrefixCache(block_size=block_size,
                                         max_entries=max_prefix_cache_entries,
                                         allocator=self.allocator)

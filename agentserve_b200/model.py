@@ -193,6 +193,7 @@ class B200LlamaModel(nn.Module):
         # True: a paged decode step whose requests share leading blocks (prefix-cache hits)
         # reads and multiplies those once per group (ops.shared_prefix_decode_attention).
         # Off by default: the results differ from the per-request attention's in rounding.
+        # An allocator's shared_prefix_decode switches it on for steps over that allocator.
         self.shared_prefix_decode: bool = False
         # Block reads (members - 1 times shared blocks, over all groups) that sharing must
         # save: below, the per-request launch is faster.  B200, rotation included, per
@@ -647,7 +648,8 @@ class B200LlamaModel(nn.Module):
     def _sharing(self, allocator, request_ids: Sequence[str], batch: int = 0) -> Optional[tuple]:
         """(groups, prefix_blocks, row_blocks) of the batch where its requests share enough
         leading blocks, else None.  batch > len(request_ids): padding rows of one block."""
-        if not self.shared_prefix_decode or len(request_ids) < 2:
+        if len(request_ids) < 2 or not (self.shared_prefix_decode
+                                        or allocator.shared_prefix_decode):
             return None
         known = self._prefix_groups
         rids = tuple(request_ids)

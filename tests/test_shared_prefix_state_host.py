@@ -3,10 +3,9 @@
 import gc
 import weakref
 
-import pytest
 import torch
 
-from agentserve_b200 import B200LlamaModel, DeviceBlockAllocator, ModelConfig
+from agentserve_b200 import B200Engine, B200LlamaModel, DeviceBlockAllocator, ModelConfig
 
 CFG = ModelConfig(hidden_dim=128, n_heads=2, n_kv_heads=1, n_layers=1, vocab_size=50,
                   max_seq_len=512, intermediate_size=64)
@@ -64,3 +63,26 @@ def test_the_threshold_holds_from_the_next_step(monkeypatch):
     alloc.free("b")
     alloc.allocate("b", 3)
     assert model._sharing(alloc, rids[:2]) is None  # nothing shared, whatever the threshold
+
+
+def test_an_engines_choice_does_not_reach_another_engine_on_the_model():
+    """shared_prefix_attention is the engine's, the model's own setting stays as it was."""
+    model, rids = make_model(), ["a", "b", "c"]
+    model.shared_prefix_decode = False
+    model.shared_prefix_min_saved = 1
+
+    def engine(**kw):
+        eng = B200Engine(CFG, model=model, num_cache_blocks=100, **kw)
+        ids = eng.allocator.allocate("a", 12)
+        for r in rids[1:]:
+            eng.allocator.share_blocks(r, ids[:10])
+            eng.allocator.allocate(r, 2)
+        return eng.allocator
+    first = engine(shared_prefix_attention=True)
+    assert model._sharing(first, rids) is not None
+    assert model.shared_prefix_decode is False
+    second = engine()
+    assert model._sharing(second, rids) is None
+    assert model._sharing(first, rids) is not None
+    model.shared_prefix_decode = True  # the model's setting holds for all of them
+    assert model._sharing(second, rids) is not None

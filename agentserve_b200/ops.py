@@ -7,6 +7,7 @@ CUDA device: there is no CPU path.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from dataclasses import dataclass
 from typing import Optional, Sequence
@@ -317,18 +318,23 @@ class SharedPrefixPlan:
         self.num_seqs, self.num_heads, self.num_kv_heads = num_seqs, num_heads, num_kv_heads
         self.head_dim, self.dtype, self.full_grid = head_dim, dtype, full_grid
         self.device = torch.device(device)
-        code = dtype_code(dtype)
-        n = int(N.load().as_shared_prefix_plan_ints(num_seqs, num_heads, num_kv_heads, head_dim,
-                                                    code))
-        _require(n > 0, "shared_prefix_plan: needs at least one sequence, heads a multiple of "
-                 "kv_heads and head_dim <= 256")
-        self.workspace_bytes = int(N.load().as_shared_prefix_workspace_size(
-            num_seqs, num_heads, num_kv_heads, head_dim, code))
+        sizes = (num_seqs, num_heads, num_kv_heads, head_dim, dtype_code(dtype))
         pinned = self.device.type == "cuda"
+        with self._current():
+            n = int(N.load().as_shared_prefix_plan_ints(*sizes))
+            _require(n > 0, "shared_prefix_plan: needs at least one sequence, heads a multiple "
+                     "of kv_heads and head_dim <= 256")
+            self.workspace_bytes = int(N.load().as_shared_prefix_workspace_size(*sizes))
         self._host = torch.zeros(n, dtype=torch.int32, pin_memory=pinned)
         self._header = self._host.data_ptr()
         self.ints = torch.zeros(n, dtype=torch.int32, device=self.device)
         self._copied = torch.cuda.Event() if pinned else None
+
+    def _current(self):
+        """The plan's device as the current one: the library divides the work for its SMs."""
+        if self.device.type == "cuda":
+            return torch.cuda.device(self.device)
+        return contextlib.nullcontext()
 
     def load(self, groups: Sequence[Sequence[int]], prefix_blocks: Sequence[int],
              row_blocks: Sequence[int]) -> None:
@@ -344,20 +350,18 @@ class SharedPrefixPlan:
         prefix = np.array(prefix_blocks, dtype=np.int32)
         rows = np.array(row_blocks, dtype=np.int32)
         host = np.zeros(self._host.numel(), dtype=np.int32)
-        N.check(N.load().as_shared_prefix_plan(
-            host.ctypes.data, host.size, offsets.ctypes.data, members.ctypes.data,
-            prefix.ctypes.data, len(groups), rows.ctypes.data, self.num_seqs, self.num_heads,
-            self.num_kv_heads, self.head_dim, dtype_code(self.dtype), int(self.full_grid)),
-            "as_shared_prefix_plan")
-        if self._copied is None:
-            self._host.numpy()[:] = host
-            self.ints.copy_(self._host)
-            return
-        with torch.cuda.device(self.device):
-            self._copied.synchronize()  # an earlier copy has left the pinned buffer
+        with self._current():
+            N.check(N.load().as_shared_prefix_plan(
+                host.ctypes.data, host.size, offsets.ctypes.data, members.ctypes.data,
+                prefix.ctypes.data, len(groups), rows.ctypes.data, self.num_seqs, self.num_heads,
+                self.num_kv_heads, self.head_dim, dtype_code(self.dtype), int(self.full_grid)),
+                "as_shared_prefix_plan")
+            if self._copied is not None:
+                self._copied.synchronize()  # an earlier copy has left the pinned buffer
             self._host.numpy()[:] = host
             self.ints.copy_(self._host, non_blocking=True)
-            self._copied.record()
+            if self._copied is not None:
+                self._copied.record()
 
 
 def shared_prefix_plan(groups: Sequence[Sequence[int]], prefix_blocks: Sequence[int],

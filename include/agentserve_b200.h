@@ -244,7 +244,7 @@ AS_API int as_paged_decode_attention_noalloc(void* out, const void* q, int64_t q
  * llama.py:419-469): a group's shared blocks are read and multiplied once for all its
  * members.  Results equal as_paged_decode_attention's up to rounding.
  *
- * as_shared_prefix_plan divides the work, on the host: group i of num_groups is the
+ * as_shared_prefix_plan divides the work for the current device, on the host: group i of num_groups is the
  * batch rows members[group_offsets[i] .. group_offsets[i+1]-1] whose block tables start
  * with the same prefix_blocks[i] blocks; no row may be in two groups, and rows in none
  * attend alone.  row_blocks[b] is the number of blocks row b will hold (at least its

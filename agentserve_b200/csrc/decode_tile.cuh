@@ -16,7 +16,9 @@ constexpr int kTileTokens = 16;  // tokens of a paged block
 // exponentiated against the current max m_run unless some score exceeds it by more
 // than 2^8 (one warp vote); only then is the max reduced across the 8 lanes that
 // share a head column and O, l rescaled.  p stays <= 256, well inside bf16/fp32
-// range, and l, O, m stay mutually consistent, so the result is unchanged.
+// range, and l, O, m stay mutually consistent, so the result is unchanged.  p is rounded to
+// the pool's type for the product with V, as the matrix instruction takes it; l sums it
+// unrounded.
 constexpr float kLazyMaxSlack = 8.0f;  // log2 units
 
 template <typename T, int D, int G>

@@ -21,7 +21,7 @@
 //
 // Few rows are bound by latency (a cluster barrier or a pass of few tokens costs about 1K
 // cycles: one bf16 row of 128,256 tokens, top-p, 19 us, of which the logits' bytes are 0.04),
-// many by integer instructions and shared-memory atomics (256 rows 83 us, 66 MB read twice).
+// many by integer instructions and shared-memory atomics (256 rows 84 us, 66 MB read twice).
 //
 // A row is worked on by a cluster of 1 to 8 CTAs, each holding a run of indexes, its warps
 // runs of that; they exchange totals over distributed shared memory.  Every decision
@@ -155,7 +155,7 @@ static_assert(sizeof(Queue) >= 3 * kBins * 4 && kThreads == kBins / 2, "find() s
 // weights up.  Rows outside this (values of 128 and more, NaN, cuts among the listed
 // values, u <= 0 or >= 1) take the general path.
 //
-// 64 rows of 128,256 tokens, top-p: 34 us, and 83 by the general path (fp16).  The passes
+// 64 rows of 128,256 tokens, top-p: 35 us, and 81 by the general path (fp16).  The passes
 // are bound by integer instructions (half rate), so a value's place is two
 // logic operations and a multiply-add away from its 16 bits: counts (4 bytes each) and
 // weights (8) lie in ascending magnitude, those of the negative values 0x8000 bytes after

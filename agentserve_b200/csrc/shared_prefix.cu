@@ -31,9 +31,11 @@ inline size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 // A block holds a tile of query rows and walks 32 * TG tokens at a time, K and V staged
 // in shared memory as fp32.  Scores: one token per lane, so a dot product needs no
 // shuffles and a K row read feeds RW query rows; products with V: one dimension per
-// lane.  TG > 1 gives token groups to different warps when there are few rows.  Bound by
-// FMAs and shared-memory reads: 16 fp32 sequences in two groups on 1,024 tokens 26 us; for
-// 64 bf16 sequences on 4,096 tokens 268 us where the tensor-core launches take 20.
+// lane.  TG > 1 gives token groups to different warps when there are few rows.  Bound, on
+// short parts, by the round of each 32 * TG tokens: ids, then K / V with no load in flight over
+// the arithmetic, and three block barriers (16 fp32 sequences in two groups on 1,024 tokens
+// 26 us, of which FMAs are 2); on long ones by FMAs and shared-memory reads: 64 bf16 sequences
+// on 4,096 tokens 209 us where the tensor-core launches take 20.
 // ===========================================================================
 constexpr int kThreads = 256;
 constexpr int kNWarps = kThreads / 32;
@@ -245,13 +247,13 @@ sp_generic_kernel(T* __restrict__ out, const T* __restrict__ q, const T* __restr
 
 constexpr int kGenericRows = 32;
 // Fixed costs of a block, in the units of its piece: halves of a 128-key tile, and blocks of
-// 16 keys.  Measured, us per call (n sequences on their shared tokens): prefix 5, with 2 the
-// same everywhere, with 10 256 on 30,000 249 instead of 203; own 16, with 32 the same, with
-// 6 64 on 4,096 28 instead of 21 and on 14,336 40 instead of 34.
+// 16 keys.  Measured, us per call (n sequences on their shared tokens): prefix 5, with 2 and
+// with 10 the same within 1%; own 16, with 32 the same, with 6 64 on 4,096 26.5 instead of 19.9
+// and on 14,336 39.3 instead of 33.3.
 constexpr int64_t kPrefixOverhead = 5;
 constexpr int64_t kOwnOverhead = 16;
 // Least own blocks of an item, where a row has that many: with 4, 16 fp32 sequences on 1,024
-// take 34 us instead of 27; with 16 as with 8.
+// take 33.7 us instead of 25.8; with 16 as with 8.
 constexpr int64_t kMinOwn = 8;
 // Most blocks of a row: its keys are counted in 31 bits.
 constexpr int kMostBlocks = (1 << 27) - 1;

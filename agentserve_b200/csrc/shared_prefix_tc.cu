@@ -9,14 +9,22 @@
 // stream is ready, warps 2-5 and 6-9 the streams' softmax, one row per thread, the two
 // warps of an SM sub-partition taking turns on its exponent unit.  Bound at head_dim 64 by
 // that unit (2,770 cycles for two streams' 128 keys; 2,048 at its peak), at 128 by the tensor
-// pipe (60% busy, S at N = 64) and the softmax's chain: 126 GFLOP in 164 us, 770 TFLOP/s.
+// pipe (60% busy, S at N = 64) and the softmax's chain: 126 GFLOP in 162 us, 778 TFLOP/s.
 //
 // Own launch (sp_own_kernel).  One sequence, up to 8 query heads of a KV head: too few
 // rows for tcgen05, and bound by reading K / V once; the decode kernel's warp-level
 // m16n8k16 fold over TMA-staged blocks (decode_tile.cuh).  Its blocks start while the
 // prefix launch runs, and join the parts (shared_prefix.cuh) after it.  300 MB of own K / V
-// in 61 us, 4.9 TB/s.  Both launches: 64 sequences on 4,096 tokens (head_dim 64) 19.8 us, on
-// 14,336 33.4; 256 on 30,000 (128) 191.
+// in 59 us, 5.1 TB/s.  The launches alone and cold, and both in a graph, us: 64 sequences on
+// 4,096 tokens (head_dim 64) 12.3, 15.4, 19.9; on 14,336 20.9, 22.3, 33.4; 256 on 30,000 (128)
+// 162, 59, 192.  Those are with the plan's own grid; full_grid adds blocks without work, which
+// come before a later head's and hold their places: 29.8, 42.8 and 211 us in all.
+//
+// Scores, softmax sums, parts and joins are fp32.  Probabilities are rounded to the pool's type
+// for the product with V, as the matrix instructions take them: by at most 2^-8 (bf16) or 2^-11
+// (fp16) of each, and in fp16 by 2^-25 of a part's largest where they are smaller than 2^-14 of
+// it.  The sums l take them unrounded.  Against 64 bits the output's error is 1.15 to 1.4 times
+// (rms) that of a result rounded once.
 //
 // Every wait is bounded: one that runs out sets status bit 4, the block stops issuing,
 // lets its copies land, frees its TMEM and leaves an empty part.
@@ -57,8 +65,8 @@ struct PreCfg {
   static constexpr int kThreads = 320;
   // TMEM columns of a stream, from 256 i: S, P (16-bit pairs), O the last D.  At D = 128
   // two S of 64 keys take turns, so that the next one is ready when a softmax ends, and P
-  // overwrites the S it came from, by then in registers.  (One S of 128 keys under its P,
-  // the next issued after PV: 256 sequences on 30,000 tokens 227 us instead of 209.)
+  // overwrites the S it came from, by then in registers.  (Before that one S of 128 keys
+  // under its P, the next issued after PV: 256 sequences on 30,000 tokens 227 us, then 209.)
   static constexpr int kCols = 512;
   static constexpr bool kAliasP = D == 128;
   static constexpr int kColP = kAliasP ? 0 : kBN;
@@ -225,7 +233,7 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
   if (warp == 1) {
     // ----------------------------------------------------------------- MMAs
     // An MMA costs this thread 20 cycles; under a branch on lane == 0 it cost 77, and the
-    // issue bound the launch (256 sequences on 30,000 tokens 243 us instead of 209).
+    // issue bound the launch (256 sequences on 30,000 tokens 243 us, by this alone 227).
     if (tc::elect_one()) {
       auto issue_s = [&](int i, int st, int place) {
         const uint32_t qi = sQ + i * Cfg::kQBytes;
@@ -377,7 +385,7 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
           f2_unpack(f2_fma(f2_pack(x[2 * c], x[2 * c + 1]), sc2, nm2), e0, e1);
           const float p0 = fast_exp2(e0), p1 = fast_exp2(e1);
           sum2[c & 3] = f2_add(sum2[c & 3], f2_pack(p0, p1));
-          pk[c] = pack2<T>(p0, p1);
+          pk[c] = pack2<T>(p0, p1);  // rounded for the product with V: see the top
           if (c == BN / 4 - 1) {  // half-way: the partner's start overlaps the rest
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->turn[1 - i][quad]);
@@ -482,7 +490,8 @@ sp_prefix_kernel(const __grid_constant__ CUtensorMap tmap_k,
 template <int D>
 struct OwnCfg {
   // Consumers; one more warp loads.  At D = 128 three and one stage, so that a block fits
-  // beside one of the prefix launch (four and two: 209 us instead of 201, as above).
+  // beside one of the prefix launch (256 sequences on 30,000 tokens, with four and two 209 us,
+  // then 201).
   static constexpr int kWarps = D == 64 ? 4 : 3;
   static constexpr int kThreads = (kWarps + 1) * 32;
   static constexpr int kSub = D / 64;

@@ -200,7 +200,7 @@ class B200LlamaModel(nn.Module):
         # layer, fused against shared: 16 sequences on 64 blocks (960 saved) 12.7 / 16.7 us
         # at head_dim 64 and 18.8 / 20.2 at 128; on 128 (1,920) 18.3 / 18.4 and 31.9 /
         # 22.9; 64 on 32 (2,016) 22.8 / 23.0 and 40.2 / 28.7; 64 on 256 61.4 / 28.8 and
-        # 113 / 36.8.
+        # 113 / 36.8.  (Of a captured step, whose full_grid plan costs 4 to 10 us of these.)
         self.shared_prefix_min_saved: int = 1920
         # (weak reference to the allocator, its epoch, requests, groups, shared blocks)
         self._prefix_groups: Optional[tuple] = None

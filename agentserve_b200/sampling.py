@@ -3,8 +3,11 @@
 AgentServe samples one request at a time with torch's global generator
 (agentserve/engine/sampling.py, engine.py:321, 379-383).  Here a whole batch is sampled
 in one launch (ops.sample_tokens) from uniform numbers that are a function of (seed,
-request, token index): a request's tokens do not depend on the batch it runs in, on the
-scheduler, or on whether its step was queued ahead.
+request, token index): the numbers do not depend on the batch, on the scheduler, or on
+whether a step was queued ahead, and equal logits give equal tokens.  The logits of a
+16-bit model do depend on the batch in their last bits (its size chooses the projections'
+kernels, and whether prefixes are shared the attention's), so a draw next to a border may
+differ there; whole runs are reproduced over batch sizes in fp32.
 """
 
 from __future__ import annotations
@@ -18,7 +21,9 @@ import numpy as np
 
 @dataclass(frozen=True)
 class SamplingParams:
-    """temperature <= 1e-6: greedy.  top_k <= 0, top_p >= 1 and min_p <= 0 are off."""
+    """temperature <= 1e-6 (or NaN): greedy, and nothing else is read.  Otherwise it is finite,
+    top_k a whole number (0 and below: off), top_p in (0, 1] (1: off) and min_p in [0, 1]
+    (0: off); other values raise ValueError."""
     temperature: float = 1.0
     top_k: int = 0
     top_p: float = 1.0

@@ -385,15 +385,16 @@ AS_API int as_greedy_argmax(int64_t* out, const void* logits, int64_t row_stride
  *         (n_k when top_p >= 1 or NaN),
  *   n_m = the number of tokens with w >= min_p (all when min_p <= 0 or NaN).
  * out[r] is the first kept token, in index order, at which the running sum of kept
- * weights exceeds u[r] times their total; a u outside [0, 1) gives the first or last
- * kept token of positive weight.  A temperature <= 1e-6 (or NaN) gives
+ * weights exceeds u[r] times their total; a u <= 0 (or NaN) gives the first kept token of
+ * positive weight, a u >= 1 the last.  A temperature <= 1e-6 (or NaN) gives
  * the first maximum, as as_greedy_argmax.  logprobs[r] (NULL to skip) is the log of the
  * token's weight over the kept total, 0 for a row that keeps one token.
  * u, temperature, top_p, min_p fp32 and top_k int32 are [num_rows]; top_k, top_p and
  * min_p may be NULL (off).  Weights are computed in 64 bits and summed in units of 2^-42 of
  * the row's largest weight, so the result does not depend on the launch; a token below
- * 2^-43 of the largest adds nothing to a sum, and no u inside (0, 1) draws it.  No
- * workspace.  vocab <= 2^20. */
+ * 2^-43 of the largest adds nothing to a sum, and no u inside (0, 1) draws it (beside its
+ * rounding to fp32, a log-probability is off by at most vocab * 2^-43).  No workspace.
+ * vocab <= 2^20. */
 AS_API int as_sample_tokens(int64_t* out, float* logprobs, const void* logits,
                             int64_t row_stride, const float* u, const float* temperature,
                             const int32_t* top_k, const float* top_p, const float* min_p,

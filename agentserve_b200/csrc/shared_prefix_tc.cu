@@ -637,9 +637,12 @@ sp_own_kernel(const __grid_constant__ CUtensorMap tmap_k,
         const uint32_t kb[1] = {smem_u32(slot)}, vb[1] = {smem_u32(slot + Cfg::kTileBytes)};
         fold_blocks<T, D, 1>(kb, vb, 1, qb, tok0, kBS, rp.len, scale_log2, m, l, o, lane,
                              Cfg::kSubBytes);
+        // Only after its own wait for the stage: a warp that runs ahead would else be counted
+        // for a round that slower ones still read.  (A warp without a block is in the last
+        // round, after which nothing is loaded.)
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[st]);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[st]);
     }
 #pragma unroll
     for (int off = 4; off < 32; off <<= 1) {

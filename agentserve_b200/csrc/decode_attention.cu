@@ -401,9 +401,12 @@ decode_fast_kernel(const __grid_constant__ CUtensorMap tmap_k,
         fold_blocks<T, D, Cfg::kFold>(kb, vb, n, qb, (blk_begin + local) * kBlockSize,
                                       kBlockSize, seq_len, scale_log2, m_run, l_run, o_acc, lane,
                                       Cfg::kSubTileBytes);
+        // Only after its own wait for the stage: a warp that runs ahead would else be counted
+        // for an earlier use of it that slower ones still read.  (Nothing is loaded after the
+        // last stage, the only one that some warps have no blocks in.)
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty_bar[st]);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty_bar[st]);
     }
     // per-head sums over the 8 lanes sharing a head column
 #pragma unroll

@@ -956,7 +956,12 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
   w.i1 = min(last, w.i0 + per_warp);
 
   cluster_started(p.C);
-  if (t == 0) s.flag = 0;
+  if (t == 0) {
+    s.flag = 0;
+    // Read where a running sum reaches its target, as every target here is at most the sum of
+    // its tokens.  Equal in all CTAs whatever happens: they must take the same barriers.
+    s.found = s.found2 = Slot{0, 0, 0};
+  }
   for (int i = t; i < kTable; i += kThreads)
     s.table[i] = exp2(double(i) / kTable) * double(1ull << kFrac);
   if constexpr (kByValue) {
@@ -1089,6 +1094,9 @@ sample_tokens_kernel(const T* __restrict__ logits, const Params p) {
         found = true;
       } else {
         w.turn = -1 - c.turn;
+        // counts by value leave masks out, so a row with -infinities comes here unsanitised;
+        // the passes below count every token
+        w.special = true;
         cluster_sync(p.C);  // no peer reads the counts any more: the queue lies over them
         w.clear();
       }

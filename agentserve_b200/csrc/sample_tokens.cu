@@ -54,6 +54,8 @@ constexpr int kMaxRun = (1 << 17) + 256;  // tokens of a CTA
 constexpr int kFrac = 42;
 constexpr int kPiece = 14;
 typedef unsigned long long u64;
+// A weight is positive in 64 bits above 2^-1075, which rounds to 0.
+constexpr double kLeastExponent = -1075.0;
 static_assert(u64(kMaxRun) << kPiece < 1ull << 32 && kFrac - 2 * kPiece <= kPiece, "sums");
 static_assert(kMaxVocab / kMaxCluster + 256 <= kMaxRun, "runs");
 
@@ -887,7 +889,7 @@ __device__ __noinline__ Cuts value_cuts(Row<__nv_bfloat16> w, ByValue& bv, int k
 }
 
 // The row's token for a u outside (0, 1): the first or last kept one whose weight is positive
-// in 64 bits (above 2^-1074).  Of the tokens at the cut those are kept before which there are
+// in 64 bits.  Of the tokens at the cut those are kept before which there are
 // fewer than `ties` in index order; `seen` of them come before this warp's run.  s.flag is 0.
 template <typename T>
 __device__ __noinline__ int end_of_kept(Row<T> w, float cut, u64 ties, u64 seen, bool last) {
@@ -903,7 +905,7 @@ __device__ __noinline__ int end_of_kept(Row<T> w, float cut, u64 ties, u64 seen,
     for (int j = 0; j < VEC; ++j) {
       const bool kept = x[j] > cut || (x[j] == cut && at < ties);
       at += x[j] == cut;
-      if (kept && (double(x[j]) - w.md) * w.c > -1074.0)
+      if (kept && (double(x[j]) - w.md) * w.c > kLeastExponent)
         best = max(best, last ? uint32_t(i + j) + 1 : ~uint32_t(i + j));
     }
     seen = __shfl_sync(0xffffffffu, upto, 31);
@@ -1350,7 +1352,7 @@ sample_small_kernel(const T* __restrict__ logits, const Params p) {
     }
     return;
   }
-  const double T64 = double(T_), one = double(1ull << kFrac);
+  const double T64 = double(T_), c = 1.4426950408889634 / T64, one = double(1ull << kFrac);
   const int n_k = k > 0 && k < V ? k : V;
   // weights in the sorted order, and how many pass min-p
   u64 w[kSmall / kThreads] = {}, sum = 0, pass = 0;
@@ -1358,11 +1360,11 @@ sample_small_kernel(const T* __restrict__ logits, const Params p) {
   for (int e = 0; e < per; ++e) {
     const int i = t * per + e;
     if (i >= n_k) break;
-    const double x = exp((double(value(i)) - double(m)) / T64);
+    const double d = double(value(i)) - double(m), x = exp(d / T64);
     w[e] = u64(__double2ll_rn(x * one));
     sum += w[e];
     pass += !(mp > 0.f) || x >= double(mp);
-    positive |= uint32_t(x > 0.0) << e;
+    positive |= uint32_t(d * c > kLeastExponent) << e;  // exp may give 0 for the smallest
   }
   const Scan ws = block_scan(sm.s, sum);
   int n = max(1, int(min(block_scan(sm.s, pass).total, u64(n_k))));

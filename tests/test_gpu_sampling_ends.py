@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 import torch
 
+from agentserve_b200 import ops
 from tests.test_gpu_sampling import DEV, check, random_logits
 
 pytestmark = pytest.mark.gpu
@@ -57,3 +58,16 @@ def test_u_of_one_with_masks_and_non_finite_logits(dtype):
     assert check(x, u, [0.8] * 5).tolist() == [2999, 99, V - 1, V - 1, 17]
     check(x, u, [0.8] * 5, k=[50] * 5, p=[0.9] * 5)
     check(x, u, [1e3] * 5, p=[0.5] * 5)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("V", [5, 1000, 3001, 30011])
+def test_the_smallest_positive_weight_counts_at_both_ends(dtype, V):
+    """e^-745 rounds to the smallest number above 0 in 64 bits, e^-745.5 to 0."""
+    x = torch.full((4, V), -1e4, device=DEV, dtype=dtype)
+    x[:, V // 2] = 0.0
+    x[0, 1] = x[1, V - 2] = -745.0
+    x[2, 1] = x[3, V - 2] = -745.5
+    u = torch.tensor([0.0, 1.0, 0.0, 1.0], device=DEV)
+    tok = ops.sample_tokens(x, u, torch.ones(4, device=DEV))
+    assert tok.tolist() == [1, V - 2, V // 2, V // 2]

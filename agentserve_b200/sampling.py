@@ -4,10 +4,10 @@ AgentServe samples one request at a time with torch's global generator
 (agentserve/engine/sampling.py, engine.py:321, 379-383).  Here a whole batch is sampled
 in one launch (ops.sample_tokens) from uniform numbers that are a function of (seed,
 request, token index): the numbers do not depend on the batch, on the scheduler, or on
-whether a step was queued ahead, and equal logits give equal tokens.  The logits of a
-16-bit model do depend on the batch in their last bits (its size chooses the projections'
-kernels, and whether prefixes are shared the attention's), so a draw next to a border may
-differ there; whole runs are reproduced over batch sizes in fp32.
+whether a step was queued ahead, and equal logits give equal tokens.  Logits may depend on
+the batch in their last bits (its size chooses the projections' kernels, and whether
+prefixes are shared the attention's), most in 16-bit types; a draw that lies that close to
+the border between two tokens may then differ.
 """
 
 from __future__ import annotations
